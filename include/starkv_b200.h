@@ -32,9 +32,10 @@
 extern "C" {
 #endif
 
-/* 3: adds starkv_prefill_attention and starkv_kv_down_cache_write (2: starkv_fold_q
- * takes a status word) */
-#define STARKV_ABI_VERSION 3
+/* 4: adds the full-rank paged cache's operators (starkv_paged_attention,
+ * starkv_page_bounds, starkv_select_pages, starkv_norm_rope); 3: starkv_prefill_attention
+ * and starkv_kv_down_cache_write; 2: starkv_fold_q takes a status word */
+#define STARKV_ABI_VERSION 4
 
 #if defined(__GNUC__)
 #define STARKV_API __attribute__((visibility("default")))
@@ -263,6 +264,120 @@ typedef struct StarKVCacheWriteArgs {
 } StarKVCacheWriteArgs;
 STARKV_API int starkv_cache_write_bf16(const StarKVCacheWriteArgs* args, void* stream);
 
+/*
+ * The full-rank paged K/V cache (the layers that a checkpoint leaves uncompressed; the
+ * reference runs its engine's stock attention there). k_cache and v_cache are
+ * [num_blocks, block_size, num_kv_heads, head_dim] with any strides {block, slot, head}
+ * (so both orders of tokens and heads), the last dimension contiguous; head_dim 64 or
+ * 128; dtype STARKV_BF16 or STARKV_F16 for all tensors of a call (else STARKV_EDTYPE).
+ * All pointers and strides give 16-byte aligned rows (else STARKV_EALIGN). block_size is
+ * any positive number. A block id outside the cache is read as block 0 and recorded as
+ * STARKV_EBOUNDS in *status (optional device int32, here and below).
+ */
+
+/*
+ * Attention of one new token per sequence:
+ *   out[b, h] = sum_t softmax_t(scale q[b, h] . K[t, h / G]) V[t, h / G],
+ * G = num_heads / num_kv_heads, over the tokens t < min(seq_lens[b], max_seq_len,
+ * max_blocks * block_size), or with `pages` (int32 [n, num_kv_heads, top], strides
+ * {sequence, head}) over the tokens of the listed pages of the block table row alone
+ * (page i holds tokens i * block_size ..; entries past min(top, pages of the sequence)
+ * are not looked at, a negative entry or one past the sequence's end holds no token, a
+ * page listed twice counts twice). A sequence without a token gives zeros. scale > 0.
+ * Cache rows past a sequence's end are not read.
+ * m_out, l_out both set: the partial form that starkv_cp_combine takes, out f32 not
+ * divided by the sum, m_out / l_out [n, num_heads] the largest scaled logit (-inf: no
+ * token) and the sum of exp(logit - m).
+ * The workspace (starkv_paged_attention_workspace_bytes, 16-byte aligned; may be null
+ * where that is 0) is scratch of this call alone: calls that can overlap need one each.
+ */
+typedef struct StarKVPagedAttnArgs {
+  const void* query;          int64_t q_stride[2];      /* [n, num_heads, head_dim] */
+  const void* k_cache;        int64_t k_stride[3];
+  const void* v_cache;        int64_t v_stride[3];
+  const int32_t* block_table; int64_t bt_stride[2];
+  const int32_t* seq_lens;
+  const int32_t* pages;       int64_t pages_stride[2];  /* null: all pages */
+  void* out;                  int64_t out_stride[2];
+  float* m_out; float* l_out;
+  int32_t* status;
+  int32_t dtype, n, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, max_seq_len, top;
+  float scale;
+} StarKVPagedAttnArgs;
+STARKV_API size_t starkv_paged_attention_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                         int32_t max_tokens);
+STARKV_API int starkv_paged_attention(const StarKVPagedAttnArgs* args, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/*
+ * Smallest and largest value of every key channel over the tokens of a page:
+ * bounds [num_blocks, num_kv_heads, {lo, hi}, head_dim] (strides {block, head}), for the
+ * pages that hold the last new_lens[b] (null: max_new) tokens of each sequence; tokens
+ * past the sequence's end do not count, other pages' bounds are left as they are. NaN
+ * keys give NaN bounds. max_new bounds new_lens on the host.
+ */
+typedef struct StarKVPageBoundsArgs {
+  const void* k_cache;        int64_t k_stride[3];
+  void* bounds;               int64_t bounds_stride[2];
+  const int32_t* block_table; int64_t bt_stride[2];
+  const int32_t* seq_lens;    const int32_t* new_lens;
+  int32_t* status;
+  int32_t dtype, n, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, max_seq_len, max_new;
+} StarKVPageBoundsArgs;
+STARKV_API int starkv_page_bounds(const StarKVPageBoundsArgs* args, void* stream);
+
+/*
+ * The `top` pages per (sequence, KV head) with the highest
+ *   sum over the head's query heads g and channels d of max(q[g,d] lo[d], q[g,d] hi[d]),
+ * ascending, -1 behind them where the sequence has fewer pages: pages int32
+ * [n, num_kv_heads, top] (strides {sequence, head}). The first `sinks` and the last
+ * `recent` pages of a sequence are always among them (sinks >= 0, recent >= 0,
+ * sinks + recent <= top); their bounds are not read. Scores in 64 bits, ties to the
+ * lowest page, a NaN score above all others. STARKV_EINVAL where the longest sequence
+ * has more than about 196,000 pages.
+ */
+typedef struct StarKVSelectPagesArgs {
+  const void* query;          int64_t q_stride[2];
+  const void* bounds;         int64_t bounds_stride[2];
+  const int32_t* block_table; int64_t bt_stride[2];
+  const int32_t* seq_lens;
+  int32_t* pages;             int64_t pages_stride[2];
+  int32_t* status;
+  int32_t dtype, n, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, max_seq_len;
+  int32_t top, sinks, recent;
+} StarKVSelectPagesArgs;
+STARKV_API int starkv_select_pages(const StarKVSelectPagesArgs* args, void* stream);
+
+/*
+ * RMS norm of each query and key head (weights [head_dim], null: none), neox rotation of
+ * the first `rot` channels by the [cos | sin] table row of the token's position (a
+ * position outside the table takes its nearest row and is recorded as STARKV_EBOUNDS),
+ * f32 inside and rounded once. query [n, num_heads, head_dim] -> q_out (may be query
+ * itself), key [n, num_kv_heads, head_dim] -> k_out (optional) and, with k_cache and
+ * v_cache set, key and value into the cache at slot_mapping (block_size * block + slot;
+ * a negative slot is not written, one past the cache is recorded and not written).
+ * num_kv_heads 0: queries alone. dtype: query, key, value and cache; w_dtype and
+ * table_dtype bf16, f16 or f32; rot a multiple of 16, at most head_dim.
+ */
+typedef struct StarKVNormRopeArgs {
+  const void* query;          int64_t q_stride[2];
+  const void* key;            int64_t k_stride[2];
+  const void* value;          int64_t v_stride[2];
+  void* q_out;                int64_t qo_stride[2];
+  void* k_out;                int64_t ko_stride[2];
+  const void* q_weight;       const void* k_weight;
+  const void* positions;
+  const void* cos_sin;        int64_t cs_stride0;
+  void* k_cache;              int64_t kc_stride[3];
+  void* v_cache;              int64_t vc_stride[3];
+  const void* slot_mapping;
+  int32_t* status;
+  int32_t dtype, w_dtype, pos_dtype, cs_dtype, slot_dtype;
+  int32_t n, num_heads, num_kv_heads, head_dim, rot, cs_rows, num_blocks, block_size;
+  float eps;
+} StarKVNormRopeArgs;
+STARKV_API int starkv_norm_rope(const StarKVNormRopeArgs* args, void* stream);
+
 /* Copy the device status word of a workspace to the host (synchronises the
  * stream; for tests and debugging, never on the decode path). Clears it when
  * reset != 0. */
@@ -281,7 +396,8 @@ STARKV_API int starkv_profile_begin(int32_t max_calls);
 STARKV_API int starkv_profile_end(float* kernel_ms /* [4] */, int32_t* calls);
 
 /* sizeof of the argument structs (0: StarKVDecodeArgs, 1: StarKVPackArgs,
- * 2: StarKVCacheWriteArgs), so a foreign-function binding can check its
+ * 2: StarKVCacheWriteArgs, 3: StarKVPagedAttnArgs, 4: StarKVPageBoundsArgs,
+ * 5: StarKVSelectPagesArgs, 6: StarKVNormRopeArgs), so a foreign-function binding can check its
  * struct layout against the library. No reference counterpart. */
 STARKV_API size_t starkv_abi_sizeof(int32_t which);
 

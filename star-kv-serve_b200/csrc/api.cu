@@ -83,6 +83,27 @@ struct Profile {
 };
 Profile g_prof;
 
+// 16-byte rows: base pointer and element strides of a 16-bit tensor
+bool rows16(const void* base, const int64_t* strides, int count) {
+  if (reinterpret_cast<uintptr_t>(base) & 15) return false;
+  for (int i = 0; i < count; ++i)
+    if (strides[i] < 0 || strides[i] % 8) return false;
+  return true;
+}
+
+// Sizes that every operator of the full-rank paged cache shares.
+int paged_cache_check(int dtype, int n, int num_kv_heads, int head_dim, int num_blocks, int block_size) {
+  if (n < 0 || num_kv_heads <= 0 || (head_dim != 64 && head_dim != 128) || num_blocks <= 0 || block_size <= 0)
+    return STARKV_EINVAL;
+  return dtype == STARKV_BF16 || dtype == STARKV_F16 ? STARKV_OK : STARKV_EDTYPE;
+}
+
+// Longest length that a call takes; 0 if the bounds are not usable.
+int paged_max_len(int max_seq_len, int max_blocks, int block_size) {
+  if (max_seq_len <= 0 || max_blocks <= 0) return 0;
+  return (int)std::min<int64_t>({max_seq_len, (int64_t)max_blocks * block_size, (int64_t)1 << 30});
+}
+
 bool is_float_dtype(int d) { return d == STARKV_BF16 || d == STARKV_F16 || d == STARKV_F32; }
 
 }  // namespace
@@ -512,6 +533,161 @@ int starkv_kv_down_cache_write(const void* hidden, int64_t h_stride0, const void
   return launch_kv_down_write(tm_w, tm_x, dp, (cudaStream_t)stream);
 }
 
+size_t starkv_paged_attention_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                              int32_t max_tokens) {
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
+      max_tokens <= starkv::paged_attn_tile_tokens())
+    return 0;
+  const size_t rows = std::min(16, num_heads / num_kv_heads);
+  return (size_t)2 * starkv::kPagedMaxShares * rows * (head_dim + 2) * sizeof(float);
+}
+
+int starkv_paged_attention(const StarKVPagedAttnArgs* a, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace starkv;
+  if (!a) return STARKV_EINVAL;
+  int st = paged_cache_check(a->dtype, a->n, a->num_kv_heads, a->head_dim, a->num_blocks, a->block_size);
+  if (st) return st;
+  const int max_len = paged_max_len(a->max_seq_len, a->max_blocks, a->block_size);
+  if (a->num_heads <= 0 || a->num_heads % a->num_kv_heads || !max_len || !(a->scale > 0.f) ||
+      !a->m_out != !a->l_out || (a->pages && a->top <= 0))
+    return STARKV_EINVAL;
+  if (a->n == 0) return STARKV_OK;
+  if (!a->query || !a->k_cache || !a->v_cache || !a->block_table || !a->seq_lens || !a->out) return STARKV_EINVAL;
+  if (!rows16(a->query, a->q_stride, 2) || !rows16(a->k_cache, a->k_stride, 3) ||
+      !rows16(a->v_cache, a->v_stride, 3) || !rows16(a->out, a->out_stride, 2))
+    return STARKV_EALIGN;
+  PagedAttnParams p{};
+  p.q = a->query; p.q_s0 = a->q_stride[0]; p.q_s1 = a->q_stride[1];
+  p.k = a->k_cache; p.k_s0 = a->k_stride[0]; p.k_s1 = a->k_stride[1]; p.k_s2 = a->k_stride[2];
+  p.v = a->v_cache; p.v_s0 = a->v_stride[0]; p.v_s1 = a->v_stride[1]; p.v_s2 = a->v_stride[2];
+  p.block_table = a->block_table; p.bt_s0 = a->bt_stride[0]; p.bt_s1 = a->bt_stride[1];
+  p.max_blocks = a->max_blocks; p.num_blocks = a->num_blocks; p.block_size = a->block_size;
+  p.page16 = a->block_size % 16 == 0;
+  p.seq_lens = a->seq_lens; p.max_len = max_len;
+  p.n = a->n; p.num_heads = a->num_heads; p.group = a->num_heads / a->num_kv_heads;
+  p.head_groups = (p.group + 15) / 16;
+  p.units = a->num_kv_heads * p.head_groups;
+  const int64_t all = ((int64_t)max_len + a->block_size - 1) / a->block_size;
+  if (a->pages) {
+    p.pages = a->pages; p.pg_s0 = a->pages_stride[0]; p.pg_s1 = a->pages_stride[1];
+    p.top = (int)std::min<int64_t>(a->top, all);
+    const int64_t tokens = p.top * (int64_t)a->block_size;
+    if (tokens > (int64_t)1 << 30) return STARKV_EINVAL;
+    p.max_unit_tokens = (int)tokens;
+  } else {
+    p.max_unit_tokens = max_len;
+  }
+  p.scale = a->scale;
+  p.out = a->out; p.o_s0 = a->out_stride[0]; p.o_s1 = a->out_stride[1];
+  p.m_out = a->m_out; p.l_out = a->l_out;
+  p.part_rows = std::min(16, p.group);
+  const size_t need = starkv_paged_attention_workspace_bytes(a->num_heads, a->num_kv_heads, a->head_dim, p.max_unit_tokens);
+  if (need && (!workspace || workspace_bytes < need)) return STARKV_EWORKSPACE;
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 15)) return STARKV_EALIGN;
+  p.part = reinterpret_cast<float*>(workspace);
+  p.status = a->status;
+  DeviceInfo dev;
+  if ((st = device_info(dev))) return st;
+  return launch_paged_attn(p, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream);
+}
+
+int starkv_page_bounds(const StarKVPageBoundsArgs* a, void* stream) {
+  using namespace starkv;
+  if (!a) return STARKV_EINVAL;
+  int st = paged_cache_check(a->dtype, a->n, a->num_kv_heads, a->head_dim, a->num_blocks, a->block_size);
+  if (st) return st;
+  const int max_len = paged_max_len(a->max_seq_len, a->max_blocks, a->block_size);
+  if (!max_len || a->max_new < 0) return STARKV_EINVAL;
+  if (a->n == 0 || a->max_new == 0) return STARKV_OK;
+  if (!a->k_cache || !a->bounds || !a->block_table || !a->seq_lens) return STARKV_EINVAL;
+  if (!rows16(a->k_cache, a->k_stride, 3) || !rows16(a->bounds, a->bounds_stride, 2)) return STARKV_EALIGN;
+  PageBoundsParams p{};
+  p.k = a->k_cache; p.k_s0 = a->k_stride[0]; p.k_s1 = a->k_stride[1]; p.k_s2 = a->k_stride[2];
+  p.bounds = a->bounds; p.b_s0 = a->bounds_stride[0]; p.b_s1 = a->bounds_stride[1];
+  p.block_table = a->block_table; p.bt_s0 = a->bt_stride[0]; p.bt_s1 = a->bt_stride[1];
+  p.max_blocks = a->max_blocks; p.num_blocks = a->num_blocks; p.block_size = a->block_size;
+  p.seq_lens = a->seq_lens; p.new_lens = a->new_lens; p.max_len = max_len;
+  p.max_new = std::min(a->max_new, max_len);
+  // pages that max_new tokens touch, wherever they begin; no more than the sequence has
+  p.max_pages = (int)std::min<int64_t>(((int64_t)p.max_new - 1 + a->block_size - 1) / a->block_size + 1,
+                                       ((int64_t)max_len + a->block_size - 1) / a->block_size);
+  p.n = a->n; p.num_kv_heads = a->num_kv_heads; p.status = a->status;
+  DeviceInfo dev;
+  if ((st = device_info(dev))) return st;
+  return launch_page_bounds(p, a->dtype, a->head_dim, (cudaStream_t)stream);
+}
+
+int starkv_select_pages(const StarKVSelectPagesArgs* a, void* stream) {
+  using namespace starkv;
+  if (!a) return STARKV_EINVAL;
+  int st = paged_cache_check(a->dtype, a->n, a->num_kv_heads, a->head_dim, a->num_blocks, a->block_size);
+  if (st) return st;
+  const int max_len = paged_max_len(a->max_seq_len, a->max_blocks, a->block_size);
+  if (a->num_heads <= 0 || a->num_heads % a->num_kv_heads || !max_len || a->top <= 0 || a->sinks < 0 ||
+      a->recent < 0 || (int64_t)a->sinks + a->recent > a->top)
+    return STARKV_EINVAL;
+  if (a->n == 0) return STARKV_OK;
+  if (!a->query || !a->bounds || !a->block_table || !a->seq_lens || !a->pages) return STARKV_EINVAL;
+  if (!rows16(a->query, a->q_stride, 2) || !rows16(a->bounds, a->bounds_stride, 2)) return STARKV_EALIGN;
+  SelectPagesParams p{};
+  p.q = a->query; p.q_s0 = a->q_stride[0]; p.q_s1 = a->q_stride[1];
+  p.bounds = a->bounds; p.b_s0 = a->bounds_stride[0]; p.b_s1 = a->bounds_stride[1];
+  p.block_table = a->block_table; p.bt_s0 = a->bt_stride[0]; p.bt_s1 = a->bt_stride[1];
+  p.max_blocks = a->max_blocks; p.num_blocks = a->num_blocks; p.block_size = a->block_size;
+  p.seq_lens = a->seq_lens; p.max_len = max_len; p.n = a->n; p.num_kv_heads = a->num_kv_heads;
+  p.group = a->num_heads / a->num_kv_heads; p.top = a->top; p.sinks = a->sinks; p.recent = a->recent;
+  p.pages = a->pages; p.pg_s0 = a->pages_stride[0]; p.pg_s1 = a->pages_stride[1];
+  p.status = a->status;
+  DeviceInfo dev;
+  if ((st = device_info(dev))) return st;
+  return launch_select_pages(p, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream);
+}
+
+int starkv_norm_rope(const StarKVNormRopeArgs* a, void* stream) {
+  using namespace starkv;
+  if (!a || a->n < 0 || a->num_heads <= 0 || a->num_kv_heads < 0 || (a->head_dim != 64 && a->head_dim != 128) ||
+      a->rot <= 0 || a->rot % 16 || a->rot > a->head_dim || a->cs_rows <= 0 || a->cs_stride0 < a->rot ||
+      !(a->eps >= 0.f))
+    return STARKV_EINVAL;
+  if (a->dtype != STARKV_BF16 && a->dtype != STARKV_F16) return STARKV_EDTYPE;
+  if (!is_float_dtype(a->cs_dtype) || ((a->q_weight || a->k_weight) && !is_float_dtype(a->w_dtype)) ||
+      (a->pos_dtype != STARKV_I32 && a->pos_dtype != STARKV_I64))
+    return STARKV_EDTYPE;
+  const bool cache = a->k_cache || a->v_cache;
+  if (cache && (!a->k_cache || !a->v_cache || !a->value || !a->slot_mapping || a->num_kv_heads == 0 ||
+                a->num_blocks <= 0 || a->block_size <= 0))
+    return STARKV_EINVAL;
+  if (cache && a->slot_dtype != STARKV_I32 && a->slot_dtype != STARKV_I64) return STARKV_EDTYPE;
+  if (a->n == 0) return STARKV_OK;
+  if (!a->query || !a->q_out || !a->positions || !a->cos_sin || (a->num_kv_heads > 0 && (!a->key || (!a->k_out && !cache))))
+    return STARKV_EINVAL;
+  const int per16 = a->cs_dtype == STARKV_F32 ? 4 : 8;
+  if (!rows16(a->query, a->q_stride, 2) || !rows16(a->q_out, a->qo_stride, 2) ||
+      (reinterpret_cast<uintptr_t>(a->cos_sin) & 15) || a->cs_stride0 % per16 ||
+      (reinterpret_cast<uintptr_t>(a->q_weight) & 15) || (reinterpret_cast<uintptr_t>(a->k_weight) & 15) ||
+      (a->num_kv_heads > 0 && !rows16(a->key, a->k_stride, 2)) || (a->k_out && !rows16(a->k_out, a->ko_stride, 2)) ||
+      (cache && (!rows16(a->value, a->v_stride, 2) || !rows16(a->k_cache, a->kc_stride, 3) ||
+                 !rows16(a->v_cache, a->vc_stride, 3))))
+    return STARKV_EALIGN;
+  NormRopeParams p{};
+  p.q = a->query; p.q_s0 = a->q_stride[0]; p.q_s1 = a->q_stride[1];
+  p.k = a->key; p.k_s0 = a->k_stride[0]; p.k_s1 = a->k_stride[1];
+  p.v = cache ? a->value : nullptr; p.v_s0 = a->v_stride[0]; p.v_s1 = a->v_stride[1];
+  p.q_out = a->q_out; p.qo_s0 = a->qo_stride[0]; p.qo_s1 = a->qo_stride[1];
+  p.k_out = a->k_out; p.ko_s0 = a->ko_stride[0]; p.ko_s1 = a->ko_stride[1];
+  p.q_weight = a->q_weight; p.k_weight = a->k_weight; p.w_dtype = a->w_dtype; p.eps = a->eps;
+  p.positions = a->positions; p.pos_dtype = a->pos_dtype;
+  p.table = a->cos_sin; p.t_s0 = a->cs_stride0; p.table_dtype = a->cs_dtype; p.table_rows = a->cs_rows; p.rot = a->rot;
+  p.k_cache = a->k_cache; p.kc_s0 = a->kc_stride[0]; p.kc_s1 = a->kc_stride[1]; p.kc_s2 = a->kc_stride[2];
+  p.v_cache = a->v_cache; p.vc_s0 = a->vc_stride[0]; p.vc_s1 = a->vc_stride[1]; p.vc_s2 = a->vc_stride[2];
+  p.num_blocks = a->num_blocks; p.block_size = a->block_size;
+  p.slots = a->slot_mapping; p.slot_dtype = a->slot_dtype;
+  p.n = a->n; p.num_heads = a->num_heads; p.num_kv_heads = a->num_kv_heads; p.status = a->status;
+  DeviceInfo dev;
+  if (const int st = device_info(dev)) return st;
+  return launch_norm_rope(p, a->dtype, a->head_dim, (cudaStream_t)stream);
+}
+
 int starkv_read_status(void* workspace, int32_t* host_status, int32_t reset, void* stream) {
   if (!workspace || !host_status) return STARKV_EINVAL;
   cudaStream_t s = (cudaStream_t)stream;
@@ -563,11 +739,15 @@ size_t starkv_abi_sizeof(int32_t which) {
     case 0: return sizeof(StarKVDecodeArgs);
     case 1: return sizeof(StarKVPackArgs);
     case 2: return sizeof(StarKVCacheWriteArgs);
+    case 3: return sizeof(StarKVPagedAttnArgs);
+    case 4: return sizeof(StarKVPageBoundsArgs);
+    case 5: return sizeof(StarKVSelectPagesArgs);
+    case 6: return sizeof(StarKVNormRopeArgs);
     default: return 0;
   }
 }
 
-const char* starkv_version(void) { return "starkv_b200 1.2 (abi 3, sm_100a)"; }
+const char* starkv_version(void) { return "starkv_b200 1.3 (abi 4, sm_100a)"; }
 
 const char* starkv_strerror(int status) {
   switch (status) {

@@ -1,0 +1,628 @@
+// Attention of one new token per sequence over a paged full-rank K/V cache:
+//   out[b, h] = sum_t softmax_t(scale q[b, h] . K[t, h / G]) V[t, h / G],  t < seq_lens[b]
+// (G = query heads per KV head), over all tokens or over a list of pages per (sequence,
+// KV head).
+//
+// What bounds it: every K and V row is read once and used for G heads, 4 G FLOP per
+// element of 2 bytes, so the cache read is the cost. The tokens of all (sequence, KV
+// head) units are laid end to end in 64-token tiles and every CTA of one wave takes an
+// equal run of them, whatever the mix of lengths. A unit that lies inside one CTA's run
+// is finished there; a unit that crosses CTA borders leaves one partial (max, sum,
+// unnormalised output) per CTA, and join_kernel adds them in the order of the CTAs, so
+// results do not depend on timing.
+//
+// A warp owns 16 tokens of each 64-token tile and a private ring of cp.async stages in
+// shared memory (no block barrier between tiles). 16 query heads are the M of
+// mma.sync.m16n8k16: S = Q K^T (B from ldmatrix), P from the accumulators' own layout,
+// O += P V (B from ldmatrix.trans). mma.sync and not tcgen05: a tile is 16 tokens x at
+// most 16 heads, the tensor pipe is idle most of the time either way, and P stays in
+// registers instead of a round trip through tensor memory. Cache rows past a sequence's
+// end are filled with zeros by the copy itself, so whatever they hold cannot reach the
+// sums. P is split into a high and a low part of the cache's type, so that its rounding
+// (2^-9 for bf16) does not show in the result; with G <= 8 both parts share one MMA (rows
+// 0-7 and 8-15), so the split costs nothing.
+#include <type_traits>
+
+#include "starkv_common.cuh"
+#include "starkv_kernels.h"
+
+namespace starkv {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kSub = 16;                 // tokens of a warp's share of a tile
+constexpr int kTileTok = kWarps * kSub;  // tokens of a tile
+constexpr int kStages = 3;
+constexpr int kMaxShares = kPagedMaxShares;
+constexpr int kRowsM = 16;               // query heads of one MMA
+
+template <int D>
+struct Ring {
+  static constexpr int row_bytes = D * 2;
+  static constexpr int op_bytes = kSub * row_bytes;      // K or V of a subtile
+  static constexpr int stage_bytes = 2 * op_bytes;
+  static constexpr int warp_bytes = kStages * stage_bytes;
+  static constexpr int bytes = kWarps * warp_bytes;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// (a, b) as two 16-bit values in one register, and what that rounding left over
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(__half, float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack2(__nv_bfloat16, uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack2(__half, uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Weights are kept times 2^kBias: f16 has no value below 2^-24, so that weights under
+// 2^-25 of the largest would leave the output but not the sum (at 131072 tokens up to
+// 2^-8 of it); times 2^10 that is 2^-18 and the largest weight, 1024, is far from f16's
+// end. The factor is the same in output and sum.
+template <typename T>
+constexpr float weight_bias() {
+  return std::is_same<T, __half>::value ? 10.f : 0.f;
+}
+
+// Tokens that a (sequence, KV head) unit of sequence b covers.
+__device__ __forceinline__ int unit_tokens(const PagedAttnParams& p, int b) {
+  const int L = min(max(p.seq_lens[b], 0), p.max_len);
+  if (!p.pages) return L;
+  return min(p.top, (L + p.block_size - 1) / p.block_size) * p.block_size;
+}
+__device__ __forceinline__ int unit_tiles(const PagedAttnParams& p, int b) {
+  return b < p.n ? (unit_tokens(p, b) + kTileTok - 1) / kTileTok : 0;
+}
+
+// Total tiles (of one unit per sequence) of the batch; every warp computes it.
+__device__ int64_t total_tiles(const PagedAttnParams& p, int lane) {
+  int64_t s = 0;
+  for (int b = lane; b < p.n; b += 32) s += unit_tiles(p, b);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  return s;
+}
+
+// The sequence that holds global tile g (tiles of `units` units each, sequences in
+// order) and the global index of its first tile. Every warp computes it.
+__device__ void find_sequence(const PagedAttnParams& p, int64_t g, int lane, int& seq, int64_t& first) {
+  int64_t base = 0;
+  for (int b0 = 0; b0 < p.n; b0 += 32) {
+    const int64_t mine = (int64_t)unit_tiles(p, b0 + lane) * p.units;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const uint32_t hit = __ballot_sync(~0u, base + incl > g);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      seq = b0 + l;
+      first = base + __shfl_sync(~0u, incl - mine, l);
+      return;
+    }
+    base += __shfl_sync(~0u, incl, 31);
+  }
+  seq = p.n;
+  first = base;
+}
+
+// f32 partials: per share two slots (its first unit, its last one) of
+// [rows][D] outputs, then [rows] max and [rows] sum.
+__device__ __forceinline__ float* part_slot(const PagedAttnParams& p, int D, int share, int which) {
+  return p.part + (int64_t)(2 * share + which) * p.part_rows * (D + 2);
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, float4 v) {
+  uint2 u;
+  u.x = pack2(T{}, v.x, v.y);
+  u.y = pack2(T{}, v.z, v.w);
+  *reinterpret_cast<uint2*>(dst) = u;
+}
+
+// Final output of query head `head` of sequence b, four channels from column c.
+// `o` unnormalised, `m` the largest raw q . k.
+template <typename T>
+__device__ __forceinline__ void store_out(const PagedAttnParams& p, int b, int head, int c, float4 o, float m, float l) {
+  const int64_t at = b * p.o_s0 + head * p.o_s1 + c;
+  if (p.m_out) {
+    constexpr float back = std::is_same<T, __half>::value ? 1.f / 1024.f : 1.f;   // 2^-weight_bias
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) =
+        make_float4(o.x * back, o.y * back, o.z * back, o.w * back);
+    if (c == 0) {
+      p.m_out[(int64_t)b * p.num_heads + head] = m * p.scale;
+      p.l_out[(int64_t)b * p.num_heads + head] = l * back;
+    }
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // no token: 0; a NaN sum stays NaN
+  store4(reinterpret_cast<T*>(p.out) + at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+}
+
+// kTwo: more than 8 query heads in the unit's MMA rows.
+template <typename T, int D, bool kTwo, bool kSparse>
+__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttnParams p) {
+  using R = Ring<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red_m[kWarps][kRowsM], red_l[kWarps][kRowsM];
+  constexpr int kChunks = D / 8;             // 16-byte pieces of a row
+  constexpr int kRowsPer = 32 / kChunks;     // rows of one warp-wide copy
+  constexpr int kKSteps = D / 16;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int qr = lane >> 2, qc = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * R::warp_bytes;
+  const float c_log2 = p.scale * 1.4426950408889634f;
+  constexpr float kBias = weight_bias<T>();
+
+  // sequences without a token have no tile: their outputs are written here
+  for (int b = blockIdx.x; b < p.n; b += gridDim.x) {
+    if (unit_tokens(p, b) > 0) continue;
+    for (int i = threadIdx.x; i < p.num_heads * (D / 4); i += kThreads)
+      store_out<T>(p, b, i / (D / 4), (i % (D / 4)) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+  }
+
+  const int64_t total = total_tiles(p, lane) * p.units;
+  const int shares = (int)min((int64_t)gridDim.x, total);
+  if ((int)blockIdx.x >= shares) return;
+  const int64_t g0 = total * blockIdx.x / shares, g1 = total * (blockIdx.x + 1) / shares;
+  int b;
+  int64_t first;
+  find_sequence(p, g0, lane, b, first);
+  int tiles = unit_tiles(p, b);
+  int unit = (int)((g0 - first) / tiles);
+  int t0 = (int)((g0 - first) % tiles);
+
+  for (int64_t g = g0; g < g1;) {
+    const int t1 = (int)min((int64_t)tiles, t0 + (g1 - g));
+    const int hk = unit / p.head_groups, hg = unit % p.head_groups;
+    const int head0 = hk * p.group + hg * kRowsM;
+    const int rows = min(kRowsM, p.group - hg * kRowsM);
+    const int L = min(max(p.seq_lens[b], 0), p.max_len);
+    const int tokens = unit_tokens(p, b);
+    const int32_t* bt = p.block_table + b * p.bt_s0;
+    const int32_t* list = kSparse ? p.pages + b * p.pg_s0 + hk * p.pg_s1 : nullptr;
+    const char* kbase = reinterpret_cast<const char*>(p.k) + hk * p.k_s2 * 2;
+    const char* vbase = reinterpret_cast<const char*>(p.v) + hk * p.v_s2 * 2;
+    // this warp's 16-token subtiles of the segment
+    int subs = t1 - t0;
+    if (subs && (t1 - 1) * kTileTok + warp * kSub >= tokens) --subs;
+    const int base0 = t0 * kTileTok + warp * kSub;
+
+    // Q as A fragments
+    uint32_t qa[kKSteps][4];
+    {
+      const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)head0 * p.q_s1;
+#pragma unroll
+      for (int kk = 0; kk < kKSteps; ++kk) {
+        const int d = kk * 16 + 2 * qc;
+        const T* r0 = q + (int64_t)qr * p.q_s1 + d;
+        const T* r1 = q + (int64_t)(qr + 8) * p.q_s1 + d;
+        qa[kk][0] = qr < rows ? *reinterpret_cast<const uint32_t*>(r0) : 0u;
+        qa[kk][2] = qr < rows ? *reinterpret_cast<const uint32_t*>(r0 + 8) : 0u;
+        qa[kk][1] = kTwo && qr + 8 < rows ? *reinterpret_cast<const uint32_t*>(r1) : 0u;
+        qa[kk][3] = kTwo && qr + 8 < rows ? *reinterpret_cast<const uint32_t*>(r1 + 8) : 0u;
+      }
+    }
+
+    // Block of the page that holds position `pos`-style index `idx` of the unit's token
+    // list, and that position (-1: not a token).
+    auto locate = [&](int idx, int& pos) -> int {
+      pos = -1;
+      if (idx >= tokens) return 0;
+      const int at = idx / p.block_size, off = idx - at * p.block_size;
+      int page = at;
+      if (kSparse) {
+        page = list[at];
+        if (page < 0 || page >= p.max_blocks) return 0;
+      }
+      const int64_t ps = (int64_t)page * p.block_size + off;
+      if (ps >= L) return 0;
+      int blk = bt[page * p.bt_s1];
+      if ((unsigned)blk >= (unsigned)p.num_blocks) {
+        record_status(p.status, STARKV_EBOUNDS);
+        blk = 0;
+      }
+      pos = (int)ps;
+      return blk;
+    };
+    // pages of whole subtiles: one lookup per subtile, 32 of them ahead by the lanes
+    int cur_blk = 0, cur_pos = -1, nxt_blk = 0, nxt_pos = -1;
+    if (p.page16) nxt_blk = locate((int)min((int64_t)base0 + lane * kTileTok, (int64_t)tokens), nxt_pos);
+
+    auto issue = [&](int i) -> uint32_t {   // returns the subtile's valid-token bits
+      const uint32_t dst = ring + (i % kStages) * R::stage_bytes;
+      const int base = base0 + i * kTileTok;
+      const int chunk = lane % kChunks, sub = lane / kChunks;
+      uint32_t valid;
+      if (p.page16) {
+        if ((i & 31) == 0) {
+          cur_blk = nxt_blk;
+          cur_pos = nxt_pos;
+          nxt_blk = locate((int)min((int64_t)base + (int64_t)(32 + lane) * kTileTok, (int64_t)tokens), nxt_pos);
+        }
+        const int blk = __shfl_sync(~0u, cur_blk, i & 31), pos = __shfl_sync(~0u, cur_pos, i & 31);
+        const int nv = pos < 0 ? 0 : min(kSub, L - pos);
+        valid = (1u << nv) - 1u;
+        const int off = pos < 0 ? 0 : pos % p.block_size;
+        const char* ks = kbase + ((int64_t)blk * p.k_s0 + (int64_t)(off + sub) * p.k_s1) * 2 + chunk * 16;
+        const char* vs = vbase + ((int64_t)blk * p.v_s0 + (int64_t)(off + sub) * p.v_s1) * 2 + chunk * 16;
+#pragma unroll
+        for (int r = 0; r < kSub; r += kRowsPer) {
+          const int row = r + sub;
+          const uint32_t o = dst + row * R::row_bytes + ((chunk ^ (row & 7)) << 4);
+          const int n = row < nv ? 16 : 0;
+          cp_async16(o, n ? ks + (int64_t)r * p.k_s1 * 2 : kbase, n);
+          cp_async16(o + R::op_bytes, n ? vs + (int64_t)r * p.v_s1 * 2 : vbase, n);
+        }
+      } else {
+        int pos;
+        const int blk = locate(base + (lane & 15), pos);
+        valid = __ballot_sync(~0u, pos >= 0) & 0xffffu;
+        const int off = pos < 0 ? 0 : pos % p.block_size;
+        const int64_t ko = ((int64_t)blk * p.k_s0 + (int64_t)off * p.k_s1) * 2;
+        const int64_t vo = ((int64_t)blk * p.v_s0 + (int64_t)off * p.v_s1) * 2;
+#pragma unroll
+        for (int r = 0; r < kSub; r += kRowsPer) {
+          const int row = r + sub;
+          const int64_t kr = __shfl_sync(~0u, ko, row), vr = __shfl_sync(~0u, vo, row);
+          const uint32_t o = dst + row * R::row_bytes + ((chunk ^ (row & 7)) << 4);
+          const int n = (valid >> row) & 1 ? 16 : 0;
+          cp_async16(o, n ? kbase + kr + chunk * 16 : kbase, n);
+          cp_async16(o + R::op_bytes, n ? vbase + vr + chunk * 16 : vbase, n);
+        }
+      }
+      return valid;
+    };
+
+    float o[2 * kKSteps][4];
+#pragma unroll
+    for (int j = 0; j < 2 * kKSteps; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+    // valid bits of the kStages - 1 = 2 subtiles in flight
+    uint32_t va = 0, vb = 0;
+    static_assert(kStages == 3, "two subtiles in flight");
+    if (subs > 0) va = issue(0);
+    cp_commit();
+    if (subs > 1) vb = issue(1);
+    cp_commit();
+    for (int i = 0; i < subs; ++i) {
+      cp_wait<kStages - 2>();
+      __syncwarp();   // every lane's copies of subtile i are in; every lane is done with subtile i - 1
+      const uint32_t valid = va;
+      va = vb;
+      if (i + 2 < subs) vb = issue(i + 2);
+      cp_commit();
+      const uint32_t kt = ring + (i % kStages) * R::stage_bytes, vt = kt + R::op_bytes;
+      const int mi = lane >> 3, rr = lane & 7;
+      // ---- S = Q K^T, 16 tokens ----
+      float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+      {
+        const int row = (mi >> 1) * 8 + rr;
+        const uint32_t a = kt + row * R::row_bytes;
+#pragma unroll
+        for (int kk = 0; kk < kKSteps; ++kk) {
+          uint32_t r[4];
+          ldsm4(a + (((2 * kk + (mi & 1)) ^ rr) << 4), r);
+          mma16816<T>(s0, qa[kk], r[0], r[1]);
+          mma16816<T>(s1, qa[kk], r[2], r[3]);
+        }
+      }
+      if (valid != 0xffffu) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (!((valid >> (2 * qc + e)) & 1)) s0[e] = s0[2 + e] = -INFINITY;
+          if (!((valid >> (8 + 2 * qc + e)) & 1)) s1[e] = s1[2 + e] = -INFINITY;
+        }
+      }
+      // ---- online softmax ----
+      float x0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1]));
+      float x1 = kTwo ? fmaxf(fmaxf(s0[2], s0[3]), fmaxf(s1[2], s1[3])) : -INFINITY;
+      x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, 1));
+      x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, 2));
+      if (kTwo) {
+        x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, 1));
+        x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, 2));
+      }
+      if (__any_sync(~0u, x0 > m0 || (kTwo && x1 > m1))) {
+        // the maxima move: what is there so far is scaled down (-inf - -inf only before the first token)
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        const float f0 = n0 == m0 ? 1.f : ex2((m0 - n0) * c_log2), f1 = n1 == m1 ? 1.f : ex2((m1 - n1) * c_log2);
+        m0 = n0;
+        m1 = n1;
+        l0 *= f0;
+        l1 *= f1;
+        const float fr = kTwo ? f1 : f0;   // G <= 8: rows 8-15 hold the low parts of rows 0-7
+#pragma unroll
+        for (int j = 0; j < 2 * kKSteps; ++j) {
+          o[j][0] *= f0;
+          o[j][1] *= f0;
+          o[j][2] *= fr;
+          o[j][3] *= fr;
+        }
+      }
+      const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+      const float p00 = ex2(fmaf(s0[0] - u0, c_log2, kBias)), p01 = ex2(fmaf(s0[1] - u0, c_log2, kBias));
+      const float p02 = ex2(fmaf(s1[0] - u0, c_log2, kBias)), p03 = ex2(fmaf(s1[1] - u0, c_log2, kBias));
+      l0 += (p00 + p01) + (p02 + p03);
+      uint32_t pa[4], pl[4];
+      pa[0] = pack2(T{}, p00, p01);
+      pa[2] = pack2(T{}, p02, p03);
+      const float2 h0 = unpack2(T{}, pa[0]), h2 = unpack2(T{}, pa[2]);
+      pl[0] = pack2(T{}, p00 - h0.x, p01 - h0.y);
+      pl[2] = pack2(T{}, p02 - h2.x, p03 - h2.y);
+      if (kTwo) {
+        const float p10 = ex2(fmaf(s0[2] - u1, c_log2, kBias)), p11 = ex2(fmaf(s0[3] - u1, c_log2, kBias));
+        const float p12 = ex2(fmaf(s1[2] - u1, c_log2, kBias)), p13 = ex2(fmaf(s1[3] - u1, c_log2, kBias));
+        l1 += (p10 + p11) + (p12 + p13);
+        pa[1] = pack2(T{}, p10, p11);
+        pa[3] = pack2(T{}, p12, p13);
+        const float2 h1 = unpack2(T{}, pa[1]), h3 = unpack2(T{}, pa[3]);
+        pl[1] = pack2(T{}, p10 - h1.x, p11 - h1.y);
+        pl[3] = pack2(T{}, p12 - h3.x, p13 - h3.y);
+      } else {
+        pa[1] = pl[0];
+        pa[3] = pl[2];
+      }
+      // ---- O += P V ----
+      {
+        const int row = (mi & 1) * 8 + rr;
+        const uint32_t a = vt + row * R::row_bytes;
+#pragma unroll
+        for (int j = 0; j < kKSteps; ++j) {
+          uint32_t r[4];
+          ldsm4_t(a + (((2 * j + (mi >> 1)) ^ rr) << 4), r);
+          mma16816<T>(o[2 * j], pa, r[0], r[1]);
+          mma16816<T>(o[2 * j + 1], pa, r[2], r[3]);
+          if (kTwo) {
+            mma16816<T>(o[2 * j], pl, r[0], r[1]);
+            mma16816<T>(o[2 * j + 1], pl, r[2], r[3]);
+          }
+        }
+      }
+    }
+    if (g + (t1 - t0) >= g1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    cp_wait<0>();
+    __syncthreads();   // no copy in flight, no warp reads its ring: the space holds the warps' outputs now
+
+    // ---- the four warps' results, added in warp order ----
+    l0 += __shfl_xor_sync(~0u, l0, 1);
+    l0 += __shfl_xor_sync(~0u, l0, 2);
+    l1 += __shfl_xor_sync(~0u, l1, 1);
+    l1 += __shfl_xor_sync(~0u, l1, 2);
+    if (qc == 0) {
+      red_m[warp][qr] = m0;
+      red_l[warp][qr] = l0;
+      red_m[warp][qr + 8] = m1;
+      red_l[warp][qr + 8] = l1;
+    }
+    float* red = reinterpret_cast<float*>(smem);   // [warp][rows][D]
+#pragma unroll
+    for (int j = 0; j < 2 * kKSteps; ++j) {
+      if (!kTwo) {
+        o[j][0] += o[j][2];
+        o[j][1] += o[j][3];
+      }
+      if (qr < rows)
+        *reinterpret_cast<float2*>(red + (warp * kRowsM + qr) * D + j * 8 + 2 * qc) = make_float2(o[j][0], o[j][1]);
+      if (kTwo && qr + 8 < rows)
+        *reinterpret_cast<float2*>(red + (warp * kRowsM + qr + 8) * D + j * 8 + 2 * qc) =
+            make_float2(o[j][2], o[j][3]);
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == tiles;
+    float* part = whole ? nullptr : part_slot(p, D, blockIdx.x, g > g0);
+    for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+      const int row = i / (D / 4), c = (i % (D / 4)) * 4;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red_m[w][row]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = red_m[w][row];
+        const float f = mw == m ? 1.f : ex2((mw - m) * c_log2);
+        const float4 v = *reinterpret_cast<const float4*>(red + (w * kRowsM + row) * D + c);
+        acc.x += f * v.x;
+        acc.y += f * v.y;
+        acc.z += f * v.z;
+        acc.w += f * v.w;
+        l += f * red_l[w][row];
+      }
+      if (whole) {
+        store_out<T>(p, b, head0 + row, c, acc, m, l);
+      } else {
+        *reinterpret_cast<float4*>(part + row * D + c) = acc;
+        if (c == 0) {
+          part[p.part_rows * D + row] = m;
+          part[p.part_rows * (D + 1) + row] = l;
+        }
+      }
+    }
+    __syncthreads();   // the space is the rings' again
+
+    g += t1 - t0;
+    t0 = 0;
+    if (g < g1 && ++unit == p.units) {
+      unit = 0;
+      do tiles = unit_tiles(p, ++b);
+      while (tiles == 0 && b < p.n);
+      if (b >= p.n) break;   // not reached: g < g1 <= total
+    }
+  }
+}
+
+// Adds the partials of the units that cross a border between shares. Block (i, row): if
+// the border after share i lies inside a unit, and share i is the unit's first, the
+// unit's shares i .. j are added, row by row; kLanes groups of threads take every
+// kLanes-th share, and their sums are added in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join_kernel(const PagedAttnParams p, int grid) {
+  constexpr int kCols = D / 4, kLanes = 256 / kCols;
+  __shared__ float sm[kLanes], sl[kLanes];
+  __shared__ float4 so[kLanes][kCols];
+  const int lane = threadIdx.x & 31;
+  const int64_t total = total_tiles(p, lane) * p.units;
+  const int shares = (int)min((int64_t)grid, total);
+  const int i0 = blockIdx.x, row = blockIdx.y;
+  int64_t u0 = 0, u1 = 0;
+  int b = 0, hk = 0, hg = 0;
+  bool mine = false;
+  if (i0 + 1 < shares) {
+    const int64_t border = total * (i0 + 1) / shares;   // first tile of share i0 + 1
+    int64_t first;
+    find_sequence(p, border, lane, b, first);
+    const int tiles = unit_tiles(p, b);
+    const int unit = (int)((border - first) / tiles);
+    u0 = first + (int64_t)unit * tiles;
+    u1 = u0 + tiles;
+    hk = unit / p.head_groups;
+    hg = unit % p.head_groups;
+    mine = u0 < border && total * i0 / shares <= u0 && row < min(kRowsM, p.group - hg * kRowsM);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the partials are written
+  if (!mine) return;
+  // share of the unit's last tile: the largest i with floor(total i / shares) <= u1 - 1
+  const int i1 = (int)((u1 * shares + total - 1) / total) - 1;
+  const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+  const float c_log2 = p.scale * 1.4426950408889634f;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = i0 + grp; i <= i1; i += kLanes) {
+    const float* part = part_slot(p, D, i, i == i0 && total * i0 / shares < u0);
+    const float pm = part[p.part_rows * D + row], pl = part[p.part_rows * (D + 1) + row];
+    const float4 v = *reinterpret_cast<const float4*>(part + row * D + col * 4);
+    const float nm = fmaxf(m, pm);
+    const float fa = m == nm ? 1.f : ex2((m - nm) * c_log2), fb = pm == nm ? 1.f : ex2((pm - nm) * c_log2);
+    acc.x = acc.x * fa + v.x * fb;
+    acc.y = acc.y * fa + v.y * fb;
+    acc.z = acc.z * fa + v.z * fb;
+    acc.w = acc.w * fa + v.w * fb;
+    l = l * fa + pl * fb;
+    m = nm;
+  }
+  so[grp][col] = acc;
+  if (col == 0) {
+    sm[grp] = m;
+    sl[grp] = l;
+  }
+  __syncthreads();
+  if (grp) return;
+  float M = -INFINITY;
+  for (int w = 0; w < kLanes; ++w) M = fmaxf(M, sm[w]);
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = 0.f;
+  for (int w = 0; w < kLanes; ++w) {
+    const float f = sm[w] == M ? 1.f : ex2((sm[w] - M) * c_log2);
+    acc.x += f * so[w][col].x;
+    acc.y += f * so[w][col].y;
+    acc.z += f * so[w][col].z;
+    acc.w += f * so[w][col].w;
+    l += f * sl[w];
+  }
+  store_out<T>(p, b, hk * p.group + hg * kRowsM + row, col * 4, acc, M, l);
+}
+
+template <typename T, int D>
+int launch_typed(const PagedAttnParams& p, int num_sms, cudaStream_t stream) {
+  const bool two = p.group > 8;
+  const void* fn = p.pages ? (two ? (const void*)paged_attn_kernel<T, D, true, true>
+                                  : (const void*)paged_attn_kernel<T, D, false, true>)
+                           : (two ? (const void*)paged_attn_kernel<T, D, true, false>
+                                  : (const void*)paged_attn_kernel<T, D, false, false>);
+  const int smem = Ring<D>::bytes;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return STARKV_ECUDA;
+  const int64_t most = (int64_t)p.n * p.units * ((p.max_unit_tokens + kTileTok - 1) / kTileTok);
+  int64_t grid = 2 * num_sms;
+  if (grid > kMaxShares) grid = kMaxShares;
+  if (grid > most) grid = most;
+  if (grid < 1) grid = 1;
+  PagedAttnParams q = p;
+  void* args[] = {&q};
+  if (cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), args, smem, stream) != cudaSuccess) return STARKV_ECUDA;
+  if (grid == 1 || p.max_unit_tokens <= kTileTok) return STARKV_OK;   // no unit has two tiles in two shares
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)grid - 1, p.part_rows);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int g = (int)grid;
+  void* jargs[] = {&q, &g};
+  if (cudaLaunchKernelExC(&cfg, (const void*)join_kernel<T, D>, jargs) != cudaSuccess) return STARKV_ECUDA;
+  return STARKV_OK;
+}
+
+}  // namespace
+
+int paged_attn_tile_tokens() { return kTileTok; }
+
+int launch_paged_attn(const PagedAttnParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream) {
+  if (dtype == STARKV_BF16)
+    return head_dim == 64 ? launch_typed<__nv_bfloat16, 64>(p, num_sms, stream)
+                          : launch_typed<__nv_bfloat16, 128>(p, num_sms, stream);
+  return head_dim == 64 ? launch_typed<__half, 64>(p, num_sms, stream)
+                        : launch_typed<__half, 128>(p, num_sms, stream);
+}
+
+}  // namespace starkv

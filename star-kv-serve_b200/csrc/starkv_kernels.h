@@ -131,6 +131,71 @@ struct DownWriteParams {
   int32_t* status;
 };
 
+// One new token per sequence over a paged full-rank cache. Strides in elements of the
+// cache type (out in the partial form: f32).
+struct PagedAttnParams {
+  const void* q; int64_t q_s0, q_s1;                 // [n, num_heads, D]
+  const void* k; int64_t k_s0, k_s1, k_s2;           // {block, slot, KV head}
+  const void* v; int64_t v_s0, v_s1, v_s2;
+  const int32_t* block_table; int64_t bt_s0, bt_s1;
+  int max_blocks, num_blocks, block_size;
+  int page16;                                        // block_size is a multiple of 16
+  const int32_t* seq_lens;
+  int max_len;                                       // longest length taken: min(max_seq_len, table's tokens)
+  const int32_t* pages; int64_t pg_s0, pg_s1;        // null: all pages; else [n, KV heads, top] page indices
+  int top;
+  int n, num_heads, group;                           // group: query heads per KV head
+  int head_groups, units;                            // ceil(group / 16); KV heads * head_groups
+  int max_unit_tokens;                               // host bound on the tokens of a unit
+  float scale;
+  void* out; int64_t o_s0, o_s1;
+  float* m_out; float* l_out;                        // set: the partial form (out f32, not divided)
+  float* part; int part_rows;                        // f32 [2 * shares][part_rows * (D + 2)]
+  int32_t* status;
+};
+constexpr int kPagedMaxShares = 384;                 // CTAs of one call at most
+
+struct PageBoundsParams {
+  const void* k; int64_t k_s0, k_s1, k_s2;
+  void* bounds; int64_t b_s0, b_s1;                  // [num_blocks, KV heads, {lo, hi}, D]
+  const int32_t* block_table; int64_t bt_s0, bt_s1;
+  int max_blocks, num_blocks, block_size;
+  const int32_t* seq_lens; const int32_t* new_lens;  // new_lens null: max_new for every sequence
+  int max_len, max_new, max_pages;                   // max_pages: pages of one sequence that max_new tokens touch
+  int n, num_kv_heads;
+  int32_t* status;
+};
+
+struct SelectPagesParams {
+  const void* q; int64_t q_s0, q_s1;
+  const void* bounds; int64_t b_s0, b_s1;
+  const int32_t* block_table; int64_t bt_s0, bt_s1;
+  int max_blocks, num_blocks, block_size;
+  const int32_t* seq_lens;
+  int max_len, n, num_kv_heads, group, top, sinks, recent;
+  int keys;                                          // score slots of one CTA (shared memory)
+  int32_t* pages; int64_t pg_s0, pg_s1;              // [n, KV heads, top]
+  int32_t* status;
+};
+
+struct NormRopeParams {
+  const void* q; int64_t q_s0, q_s1;                 // [n, num_heads, D]
+  const void* k; int64_t k_s0, k_s1;                 // [n, num_kv_heads, D]; num_kv_heads 0: queries only
+  const void* v; int64_t v_s0, v_s1;
+  void* q_out; int64_t qo_s0, qo_s1;
+  void* k_out; int64_t ko_s0, ko_s1;                 // may be null
+  const void* q_weight; const void* k_weight; int w_dtype;   // null: no norm
+  float eps;
+  const void* positions; int pos_dtype;
+  const void* table; int64_t t_s0; int table_dtype; int table_rows, rot;   // rot: rotated channels, <= D
+  void* k_cache; int64_t kc_s0, kc_s1, kc_s2;        // null: no cache write
+  void* v_cache; int64_t vc_s0, vc_s1, vc_s2;
+  int num_blocks, block_size;
+  const void* slots; int slot_dtype;
+  int n, num_heads, num_kv_heads;
+  int32_t* status;
+};
+
 size_t scores_smem_bytes(bool quant, int num_kv_heads, int n, int k_width, int code_pitch, int sc_pitch,
                          bool parts);
 int code_pitch_bytes(int bytes);
@@ -155,6 +220,11 @@ int kv_down_ctl_offset(int n_tile, int stages);
 int kv_down_split();
 int launch_kv_down_write(const CUtensorMap& tm_w, const CUtensorMap& tm_x, const DownWriteParams& p,
                          cudaStream_t stream);
+int paged_attn_tile_tokens();
+int launch_paged_attn(const PagedAttnParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
+int launch_page_bounds(const PageBoundsParams& p, int dtype, int head_dim, cudaStream_t stream);
+int launch_select_pages(SelectPagesParams p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
+int launch_norm_rope(const NormRopeParams& p, int dtype, int head_dim, cudaStream_t stream);
 int launch_prefill(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PrefillParams& p,
                    int q_tiles, cudaStream_t stream);
 

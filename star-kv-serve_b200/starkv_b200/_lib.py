@@ -76,6 +76,51 @@ class CacheWriteArgs(C.Structure):
     ]
 
 
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("query", p), ("q_stride", i64 * 2), ("k_cache", p), ("k_stride", i64 * 3), ("v_cache", p),
+        ("v_stride", i64 * 3), ("block_table", p), ("bt_stride", i64 * 2), ("seq_lens", p),
+        ("pages", p), ("pages_stride", i64 * 2), ("out", p), ("out_stride", i64 * 2),
+        ("m_out", p), ("l_out", p), ("status", p),
+        ("dtype", i32), ("n", i32), ("num_heads", i32), ("num_kv_heads", i32), ("head_dim", i32),
+        ("num_blocks", i32), ("block_size", i32), ("max_blocks", i32), ("max_seq_len", i32), ("top", i32),
+        ("scale", f32),
+    ]
+
+
+class PageBoundsArgs(C.Structure):
+    _fields_ = [
+        ("k_cache", p), ("k_stride", i64 * 3), ("bounds", p), ("bounds_stride", i64 * 2),
+        ("block_table", p), ("bt_stride", i64 * 2), ("seq_lens", p), ("new_lens", p), ("status", p),
+        ("dtype", i32), ("n", i32), ("num_kv_heads", i32), ("head_dim", i32),
+        ("num_blocks", i32), ("block_size", i32), ("max_blocks", i32), ("max_seq_len", i32), ("max_new", i32),
+    ]
+
+
+class SelectPagesArgs(C.Structure):
+    _fields_ = [
+        ("query", p), ("q_stride", i64 * 2), ("bounds", p), ("bounds_stride", i64 * 2),
+        ("block_table", p), ("bt_stride", i64 * 2), ("seq_lens", p), ("pages", p), ("pages_stride", i64 * 2),
+        ("status", p),
+        ("dtype", i32), ("n", i32), ("num_heads", i32), ("num_kv_heads", i32), ("head_dim", i32),
+        ("num_blocks", i32), ("block_size", i32), ("max_blocks", i32), ("max_seq_len", i32),
+        ("top", i32), ("sinks", i32), ("recent", i32),
+    ]
+
+
+class NormRopeArgs(C.Structure):
+    _fields_ = [
+        ("query", p), ("q_stride", i64 * 2), ("key", p), ("k_stride", i64 * 2), ("value", p), ("v_stride", i64 * 2),
+        ("q_out", p), ("qo_stride", i64 * 2), ("k_out", p), ("ko_stride", i64 * 2),
+        ("q_weight", p), ("k_weight", p), ("positions", p), ("cos_sin", p), ("cs_stride0", i64),
+        ("k_cache", p), ("kc_stride", i64 * 3), ("v_cache", p), ("vc_stride", i64 * 3),
+        ("slot_mapping", p), ("status", p),
+        ("dtype", i32), ("w_dtype", i32), ("pos_dtype", i32), ("cs_dtype", i32), ("slot_dtype", i32),
+        ("n", i32), ("num_heads", i32), ("num_kv_heads", i32), ("head_dim", i32), ("rot", i32), ("cs_rows", i32),
+        ("num_blocks", i32), ("block_size", i32), ("eps", f32),
+    ]
+
+
 EXPORTS = {
     "starkv_decode_workspace_bytes": (C.c_size_t, [i32, i32, i32, i32, i32, i32]),
     "starkv_paged_decode_bf16": (C.c_int, [C.POINTER(DecodeArgs), p, C.c_size_t, p]),
@@ -92,6 +137,11 @@ EXPORTS = {
                                              p, p]),
     "starkv_prefill_attention": (C.c_int, [p, C.POINTER(i64), p, C.POINTER(i64), p, C.POINTER(i64), i32, i32, i32, i32,
                                            i32, p, i32, i32, f32, p, C.POINTER(i64), p, p]),
+    "starkv_paged_attention_workspace_bytes": (C.c_size_t, [i32, i32, i32, i32]),
+    "starkv_paged_attention": (C.c_int, [C.POINTER(PagedAttnArgs), p, C.c_size_t, p]),
+    "starkv_page_bounds": (C.c_int, [C.POINTER(PageBoundsArgs), p]),
+    "starkv_select_pages": (C.c_int, [C.POINTER(SelectPagesArgs), p]),
+    "starkv_norm_rope": (C.c_int, [C.POINTER(NormRopeArgs), p]),
     "starkv_cache_write_bf16": (C.c_int, [C.POINTER(CacheWriteArgs), p]),
     "starkv_read_status": (C.c_int, [p, C.POINTER(i32), i32, p]),
     "starkv_status_offset": (C.c_size_t, []),
@@ -123,7 +173,8 @@ def lib() -> C.CDLL:
 
 def check_abi() -> None:
     L = lib()
-    for which, cls in enumerate((DecodeArgs, PackArgs, CacheWriteArgs)):
+    for which, cls in enumerate((DecodeArgs, PackArgs, CacheWriteArgs, PagedAttnArgs, PageBoundsArgs,
+                                 SelectPagesArgs, NormRopeArgs)):
         got = L.starkv_abi_sizeof(which)
         if got != C.sizeof(cls):
             raise RuntimeError(f"ABI mismatch for {cls.__name__}: library {got} B, binding {C.sizeof(cls)} B")
@@ -150,6 +201,31 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def same_device(what: str, **tensors) -> torch.device:
+    """The one CUDA device of the given tensors (None: left out); ValueError otherwise."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{what}: {name} must be a CUDA tensor")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, not on {dev}")
+    return dev
+
+
+def launch(what: str, device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of `device`, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        st = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    check(st, what)
 
 
 def i64s(values):

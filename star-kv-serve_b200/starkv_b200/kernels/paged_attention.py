@@ -1,0 +1,234 @@
+"""Decode attention over a paged full-rank K/V cache, whole or over selected pages, on
+the sm_100a library.
+
+The layers that a STAR-KV checkpoint leaves full-rank keep plain keys and values (the
+reference runs its engine's stock attention there). Their cache is a pair of tensors
+``[num_blocks, block_size, H_kv, head_dim]`` of any strides with a contiguous last
+dimension: tokens before heads, or heads before tokens (``empty_cache``, whose page of a
+head is one contiguous run). head_dim 64 or 128, bf16 or f16.
+
+    paged_attention_decode   one new token per sequence, split over the length and joined
+    update_page_bounds       per-page smallest / largest key channel values
+    select_pages             the pages whose bounds promise the largest scores
+    sparse_paged_decode      select_pages, then the attention over those pages alone
+
+There is no fallback: if the native library is missing the calls raise.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib, context_parallel
+
+HEAD_DIMS = (64, 128)
+_i2, _i3 = _lib.i64 * 2, _lib.i64 * 3
+
+
+def empty_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int = 128, dtype=torch.bfloat16,
+                device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """Zeroed (k_cache, v_cache) ``[num_blocks, block_size, H_kv, head_dim]`` with each
+    head's page contiguous."""
+    return tuple(torch.zeros(num_blocks, num_kv_heads, block_size, head_dim, dtype=dtype, device=device).transpose(1, 2)
+                 for _ in range(2))
+
+
+def empty_bounds(k_cache: torch.Tensor) -> torch.Tensor:
+    """Zeroed page bounds ``[num_blocks, H_kv, 2, head_dim]`` (lo, hi) of a key cache."""
+    nb, _, hkv, d = k_cache.shape
+    return torch.zeros(nb, hkv, 2, d, dtype=k_cache.dtype, device=k_cache.device)
+
+
+def _i32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.int32 else t.to(torch.int32)
+
+
+def _check_table(what: str, n: int, block_table: torch.Tensor, seq_lens: torch.Tensor):
+    if block_table.dim() != 2 or block_table.shape[0] != n or tuple(seq_lens.shape) != (n,):
+        raise ValueError(f"{what}: block_table must be [{n}, max_blocks] and seq_lens [{n}]")
+    seq_lens = _i32(seq_lens)
+    return _i32(block_table), seq_lens if seq_lens.is_contiguous() else seq_lens.contiguous()
+
+
+def _check_cache(what: str, cache: torch.Tensor, name: str, dtype: torch.dtype) -> None:
+    if cache.dim() != 4 or cache.shape[-1] not in HEAD_DIMS:
+        raise ValueError(f"{what}: {name} must be [num_blocks, block_size, H_kv, 64 or 128]")
+    if cache.dtype != dtype or dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what}: query and cache must be bf16 or f16, all the same")
+    if cache.stride(-1) != 1:
+        raise ValueError(f"{what}: {name} needs a contiguous last dimension")
+
+
+def _check_query(what: str, query: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
+    if query.dim() != 3 or query.shape[2] != head_dim or query.shape[1] == 0 or query.shape[1] % num_kv_heads:
+        raise ValueError(f"{what}: query must be [n, multiple of {num_kv_heads}, {head_dim}]")
+    if query.stride(-1) != 1:
+        raise ValueError(f"{what}: query needs a contiguous last dimension")
+
+
+def paged_attention_decode(
+    query: torch.Tensor,          # [n, H_q, head_dim], rotation applied
+    k_cache: torch.Tensor,        # [num_blocks, block_size, H_kv, head_dim]
+    v_cache: torch.Tensor,        # the same shape
+    block_table: torch.Tensor,    # [n, max_blocks] int32
+    seq_lens: torch.Tensor,       # [n] int32, including the token just written
+    max_seq_len: int,             # host-side bound on seq_lens (longer sequences are cut to it)
+    scale: float,
+    *,
+    pages: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    return_partial: bool = False,
+    partial: torch.Tensor | None = None,
+    ws: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+):
+    """``out[b, h] = softmax_t(scale q[b, h] . K[t]) V[t]`` over sequence b's tokens, query
+    head h reading KV head h // (H_q / H_kv): [n, H_q, head_dim] in the cache's dtype. A
+    sequence of length 0 gives zeros.
+
+    ``pages`` (int32 [n, H_kv, top], as ``select_pages`` returns them): attend to the
+    tokens of these pages of the sequence alone. A negative entry holds no token; each
+    listed page counts once per listing.
+
+    ``return_partial``: ``(out, m, l)`` for ``context_parallel.combine`` - out f32
+    undivided, m / l f32 [n, H_q] the largest logit and the sum of exp(logit - m) - as
+    views of one packed buffer (``partial``, allocated when not given; with head_dim 64,
+    which ``combine`` does not take, three tensors).
+
+    ``ws``: scratch of this call alone (``workspace_bytes``); by default it is
+    allocated on the current stream, so that calls that overlap, or captured graphs
+    that are replayed at once, do not share it."""
+    what = "paged_attention_decode"
+    _check_cache(what, k_cache, "k_cache", query.dtype)
+    _check_cache(what, v_cache, "v_cache", query.dtype)
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"{what}: k_cache and v_cache must have the same shape")
+    nb, bs, hkv, d = k_cache.shape
+    _check_query(what, query, hkv, d)
+    n, hq, _ = query.shape
+    block_table, seq_lens = _check_table(what, n, block_table, seq_lens)
+    top, pg = 0, (0, 0)
+    if pages is not None:
+        if pages.dim() != 3 or pages.shape[:2] != (n, hkv) or pages.dtype != torch.int32 or pages.shape[2] == 0:
+            raise ValueError(f"{what}: pages must be int32 [{n}, {hkv}, top]")
+        if pages.stride(-1) != 1:
+            raise ValueError(f"{what}: pages needs a contiguous last dimension")
+        top, pg = pages.shape[2], pages.stride()[:2]
+    m = l = None
+    if return_partial:
+        if d == 128:
+            out, m, l = context_parallel.partial_views(n, hq, query.device, partial)
+        elif partial is not None:
+            raise ValueError(f"{what}: the packed partial buffer holds head_dim 128")
+        else:
+            out = torch.empty((n, hq, d), dtype=torch.float32, device=query.device)
+            m, l = torch.empty((2, n, hq), dtype=torch.float32, device=query.device).unbind(0)
+    elif out is None:
+        out = torch.empty((n, hq, d), dtype=query.dtype, device=query.device)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1:
+        raise ValueError(f"{what}: out must be [{n}, {hq}, {d}] in the cache's dtype, last dimension contiguous")
+    dev = _lib.same_device(what, query=query, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
+                           seq_lens=seq_lens, pages=pages, out=out, ws=ws, status=status)
+    if n == 0:
+        return (out, m, l) if return_partial else out
+    lib = _lib.lib()
+    if ws is None:
+        ws = torch.empty(workspace_bytes(hq, hkv, d, top * bs if top else int(max_seq_len)), dtype=torch.uint8,
+                         device=dev)
+    a = _lib.PagedAttnArgs(
+        query.data_ptr(), _i2(*query.stride()[:2]), k_cache.data_ptr(), _i3(*k_cache.stride()[:3]),
+        v_cache.data_ptr(), _i3(*v_cache.stride()[:3]), block_table.data_ptr(), _i2(*block_table.stride()),
+        seq_lens.data_ptr(), None if pages is None else pages.data_ptr(), _i2(*pg), out.data_ptr(),
+        _i2(*out.stride()[:2]), _lib.ptr(m), _lib.ptr(l), _lib.ptr(status), _lib.dtype_code(query), n, hq, hkv, d, nb, bs,
+        block_table.shape[1], int(max_seq_len), top, float(scale))
+    _lib.launch(what, dev, lib.starkv_paged_attention, a, ws.data_ptr(), ws.numel() * ws.element_size())
+    return (out, m, l) if return_partial else out
+
+
+def workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int, max_tokens: int) -> int:
+    """Scratch of one ``paged_attention_decode`` over at most ``max_tokens`` tokens per sequence."""
+    return int(_lib.lib().starkv_paged_attention_workspace_bytes(num_heads, num_kv_heads, head_dim,
+                                                                  min(int(max_tokens), 1 << 30)))
+
+
+def update_page_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                       max_seq_len: int, *, max_new: int = 1, new_lens: torch.Tensor | None = None,
+                       status: torch.Tensor | None = None) -> None:
+    """``bounds[block, h] = (min, max)`` over the page's tokens of every channel of key head
+    h, for the pages that hold each sequence's last ``max_new`` tokens (``new_lens``: int32
+    [n], per sequence, at most max_new). Call it after those tokens are written: with
+    max_new=1 after a decode step, with the longest prompt after a prefill. Other pages'
+    bounds stay as they are."""
+    what = "update_page_bounds"
+    _check_cache(what, k_cache, "k_cache", k_cache.dtype)
+    nb, bs, hkv, d = k_cache.shape
+    if bounds.shape != (nb, hkv, 2, d) or bounds.dtype != k_cache.dtype or bounds.stride(-1) != 1 \
+            or bounds.stride(-2) != d:
+        raise ValueError(f"{what}: bounds must be [{nb}, {hkv}, 2, {d}] in the cache's dtype, (lo, hi) contiguous")
+    n = block_table.shape[0]
+    block_table, seq_lens = _check_table(what, n, block_table, seq_lens)
+    if new_lens is not None:
+        if tuple(new_lens.shape) != (n,):
+            raise ValueError(f"{what}: new_lens must be [{n}]")
+        new_lens = _i32(new_lens).contiguous()
+    dev = _lib.same_device(what, k_cache=k_cache, bounds=bounds, block_table=block_table, seq_lens=seq_lens,
+                           new_lens=new_lens, status=status)
+    a = _lib.PageBoundsArgs(
+        k_cache.data_ptr(), _i3(*k_cache.stride()[:3]), bounds.data_ptr(), _i2(*bounds.stride()[:2]),
+        block_table.data_ptr(), _i2(*block_table.stride()), seq_lens.data_ptr(), _lib.ptr(new_lens), _lib.ptr(status),
+        _lib.dtype_code(k_cache), n, hkv, d, nb, bs, block_table.shape[1], int(max_seq_len), int(max_new))
+    _lib.launch(what, dev, _lib.lib().starkv_page_bounds, a)
+
+
+def select_pages(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                 max_seq_len: int, block_size: int, top: int, *, sinks: int = 1, recent: int = 1,
+                 out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """The ``top`` pages per sequence and KV head with the largest
+    ``sum_{g, d} max(q[g, d] lo[d], q[g, d] hi[d])`` over the head's query heads g:
+    int32 [n, H_kv, top], ascending, -1 behind them where a sequence has fewer pages.
+    The first ``sinks`` and the last ``recent`` pages are always among them (the last
+    page is usually not full, and its bounds need not be up to date while recent >= 1).
+    Scores in 64 bits; ties go to the lowest page; a NaN score ranks above all others."""
+    what = "select_pages"
+    if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.shape[3] not in HEAD_DIMS:
+        raise ValueError(f"{what}: bounds must be [num_blocks, H_kv, 2, 64 or 128]")
+    nb, hkv, _, d = bounds.shape
+    if bounds.dtype != query.dtype or query.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what}: query and bounds must be bf16 or f16, both the same")
+    if bounds.stride(-1) != 1 or bounds.stride(-2) != d:
+        raise ValueError(f"{what}: the (lo, hi) rows of bounds must be contiguous")
+    _check_query(what, query, hkv, d)
+    n, hq, _ = query.shape
+    if top < 1 or sinks < 0 or recent < 0 or sinks + recent > top:
+        raise ValueError(f"{what}: need top >= 1 and sinks + recent <= top")
+    block_table, seq_lens = _check_table(what, n, block_table, seq_lens)
+    if out is None:
+        out = torch.empty((n, hkv, top), dtype=torch.int32, device=query.device)
+    elif tuple(out.shape) != (n, hkv, top) or out.dtype != torch.int32 or out.stride(-1) != 1:
+        raise ValueError(f"{what}: out must be int32 [{n}, {hkv}, {top}], last dimension contiguous")
+    dev = _lib.same_device(what, query=query, bounds=bounds, block_table=block_table, seq_lens=seq_lens, out=out,
+                           status=status)
+    if n == 0:
+        return out
+    a = _lib.SelectPagesArgs(
+        query.data_ptr(), _i2(*query.stride()[:2]), bounds.data_ptr(), _i2(*bounds.stride()[:2]),
+        block_table.data_ptr(), _i2(*block_table.stride()), seq_lens.data_ptr(), out.data_ptr(), _i2(*out.stride()[:2]),
+        _lib.ptr(status), _lib.dtype_code(query), n, hq, hkv, d, nb, int(block_size), block_table.shape[1],
+        int(max_seq_len), int(top), int(sinks), int(recent))
+    _lib.launch(what, dev, _lib.lib().starkv_select_pages, a)
+    return out
+
+
+def sparse_paged_decode(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bounds: torch.Tensor,
+                        block_table: torch.Tensor, seq_lens: torch.Tensor, max_seq_len: int, scale: float, top: int,
+                        *, sinks: int = 1, recent: int = 1, out: torch.Tensor | None = None,
+                        ws: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """``select_pages``, then ``paged_attention_decode`` over those pages: (out, pages).
+    ``bounds`` as ``update_page_bounds`` keeps them. With top >= the pages of a sequence
+    this is the attention over all of it."""
+    if bounds.shape[:2] != (k_cache.shape[0], k_cache.shape[2]):
+        raise ValueError("sparse_paged_decode: bounds and cache must have the same blocks and heads")
+    pages = select_pages(query, bounds, block_table, seq_lens, max_seq_len, k_cache.shape[1], top, sinks=sinks,
+                         recent=recent, status=status)
+    out = paged_attention_decode(query, k_cache, v_cache, block_table, seq_lens, max_seq_len, scale, pages=pages,
+                                 out=out, ws=ws, status=status)
+    return out, pages

@@ -1,0 +1,118 @@
+"""Per-head RMS norms of queries and keys, their rotation and the write of keys and values
+into a paged full-rank cache, in one launch of the sm_100a library.
+
+    y = x * rsqrt(mean(x^2) + eps) * weight      (no weight: y = x)
+    out = neox rotation of y by the [cos | sin] row of the token's position
+
+Inside all of it is f32 and rounded once. The rotated width is the table's width (a
+multiple of 16, at most head_dim); channels behind it are passed through. There is no
+fallback: if the native library is missing the calls raise.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from .paged_attention import HEAD_DIMS, _check_cache
+
+_i2, _i3 = _lib.i64 * 2, _lib.i64 * 3
+_Z2, _Z3 = _i2(0, 0), _i3(0, 0, 0)
+
+
+def _rows(what: str, name: str, t: torch.Tensor, n: int, heads: int, d: int, dtype) -> None:
+    if t.dim() != 3 or tuple(t.shape) != (n, heads, d) or t.dtype != dtype or t.stride(-1) != 1:
+        raise ValueError(f"{what}: {name} must be [{n}, {heads}, {d}] in the query's dtype, last dimension contiguous")
+
+
+def _run(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping, q_weight, k_weight, eps, q_out, k_out,
+         status):
+    if q.dim() != 3 or q.shape[2] not in HEAD_DIMS or q.shape[1] == 0:
+        raise ValueError(f"{what}: q must be [n, heads, 64 or 128]")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what}: q, k and v must be bf16 or f16")
+    n, hq, d = q.shape
+    _rows(what, "q", q, n, hq, d, q.dtype)
+    hkv = 0
+    if k is not None:
+        hkv = k.shape[1] if k.dim() == 3 else 0
+        if hkv == 0:
+            raise ValueError(f"{what}: k must be [n, KV heads, {d}]")
+        _rows(what, "k", k, n, hkv, d, q.dtype)
+    if positions.shape != (n,) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: positions must be int32 or int64 [{n}]")
+    if cos_sin_cache.dim() != 2 or cos_sin_cache.stride(-1) != 1 or cos_sin_cache.shape[1] % 16 or \
+            not 0 < cos_sin_cache.shape[1] <= d:
+        raise ValueError(f"{what}: cos_sin_cache must be [positions, rot], rot a multiple of 16 and at most {d}")
+    w_dtype = 0
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            if tuple(w.shape) != (d,) or not w.is_contiguous():
+                raise ValueError(f"{what}: {name} must be a contiguous [{d}]")
+            w_dtype = _lib.dtype_code(w)
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"{what}: q_weight and k_weight must share one dtype")
+    nb = bs = slot_dtype = 0
+    if k_cache is not None:
+        _check_cache(what, k_cache, "k_cache", q.dtype)
+        _check_cache(what, v_cache, "v_cache", q.dtype)
+        if k_cache.shape != v_cache.shape or k_cache.shape[2:] != (hkv, d):
+            raise ValueError(f"{what}: k_cache and v_cache must both be [num_blocks, block_size, {hkv}, {d}]")
+        _rows(what, "v", v, n, hkv, d, q.dtype)
+        if slot_mapping.shape != (n,) or slot_mapping.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{what}: slot_mapping must be int32 or int64 [{n}]")
+        nb, bs = k_cache.shape[:2]
+        slot_mapping, slot_dtype = slot_mapping.contiguous(), _lib.dtype_code(slot_mapping)
+    if q_out is None:
+        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    else:
+        _rows(what, "q_out", q_out, n, hq, d, q.dtype)
+    if k_out is not None:
+        _rows(what, "k_out", k_out, n, hkv, d, q.dtype)
+    positions = positions.contiguous()
+    dev = _lib.same_device(what, q=q, k=k, v=v, positions=positions, cos_sin_cache=cos_sin_cache, k_cache=k_cache,
+                           v_cache=v_cache, slot_mapping=slot_mapping, q_weight=q_weight, k_weight=k_weight,
+                           q_out=q_out, k_out=k_out, status=status)
+    if n == 0:
+        return q_out
+    P = _lib.ptr
+    a = _lib.NormRopeArgs(
+        q.data_ptr(), _i2(*q.stride()[:2]), P(k), _Z2 if k is None else _i2(*k.stride()[:2]),
+        P(v), _Z2 if v is None else _i2(*v.stride()[:2]), q_out.data_ptr(), _i2(*q_out.stride()[:2]),
+        P(k_out), _Z2 if k_out is None else _i2(*k_out.stride()[:2]), P(q_weight), P(k_weight),
+        positions.data_ptr(), cos_sin_cache.data_ptr(), cos_sin_cache.stride(0),
+        P(k_cache), _Z3 if k_cache is None else _i3(*k_cache.stride()[:3]),
+        P(v_cache), _Z3 if v_cache is None else _i3(*v_cache.stride()[:3]), P(slot_mapping), P(status),
+        _lib.dtype_code(q), w_dtype, _lib.dtype_code(positions), _lib.dtype_code(cos_sin_cache), slot_dtype,
+        n, hq, hkv, d, cos_sin_cache.shape[1], cos_sin_cache.shape[0], nb, bs, float(eps))
+    _lib.launch(what, dev, _lib.lib().starkv_norm_rope, a)
+    return q_out
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos_sin_cache: torch.Tensor, *,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None):
+    """(q_out, k_out): normed and rotated q [n, H_q, head_dim] and k [n, H_kv, head_dim]
+    (k None: q alone, k_out None). q_out / k_out may be q / k themselves. A position
+    outside the table takes the nearest row and is recorded in ``status``."""
+    if k is None and (k_out is not None or k_weight is not None):
+        raise ValueError("qk_norm_rope: k_out and k_weight need k")
+    if k is not None and k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out = _run("qk_norm_rope", q, k, None, positions, cos_sin_cache, None, None, None, q_weight, k_weight, eps, q_out,
+                 k_out, status)
+    return q_out, k_out
+
+
+def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                       cos_sin_cache: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       slot_mapping: torch.Tensor, *, q_weight: torch.Tensor | None = None,
+                       k_weight: torch.Tensor | None = None, eps: float = 1e-6, q_out: torch.Tensor | None = None,
+                       k_out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Normed and rotated q; the normed, rotated k and v go to
+    ``cache[slot // block_size, slot % block_size]`` (and k to ``k_out`` where given, as a
+    prefill needs it). A negative slot is not written; a slot past the cache is not written
+    and recorded in ``status``. Slots are distinct: of two tokens with the same slot either
+    may stay. q_out may be q itself."""
+    return _run("qk_norm_rope_write", q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping, q_weight,
+                k_weight, eps, q_out, k_out, status)

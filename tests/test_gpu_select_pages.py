@@ -1,0 +1,176 @@
+"""GPU checks of the page bounds (exact: smallest and largest value) and of the page
+selection, whose result is compared as whole numbers with a float64 sort of
+sum_{g, d} max(q lo, q hi), ties to the lowest page."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return torch.device("cuda", 0)
+
+
+def table(n, per, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randperm(n * per, generator=g) + 1).view(n, per).int().to(cuda())
+
+
+def expected(q, bounds, bt, lens, bs, top, sinks, recent):
+    n, H, D = q.shape
+    Hkv = bounds.shape[1]
+    G = H // Hkv
+    out = torch.full((n, Hkv, top), -1, dtype=torch.int32)
+    for b in range(n):
+        P = -(-int(lens[b]) // bs)
+        for h in range(Hkv):
+            if P <= top:
+                out[b, h, :P] = torch.arange(P)
+                continue
+            B = bounds[bt[b, :P].long(), h].double()
+            Q = q[b, h * G:(h + 1) * G].double()
+            s = torch.maximum(Q[:, None] * B[:, 0], Q[:, None] * B[:, 1]).sum((0, 2))
+            s = torch.where(s.isnan(), float("inf"), s)
+            keep = list(range(sinks)) + list(range(P - recent, P))
+            rest = [i for i in torch.argsort(s, descending=True, stable=True).tolist() if i not in set(keep)]
+            out[b, h] = torch.tensor(sorted(keep + rest[:top - len(keep)]), dtype=torch.int32)
+    return out
+
+
+def run(lens, H, Hkv, D=128, bs=16, top=8, sinks=1, recent=1, dtype=torch.bfloat16, seed=0, levels=None, zero_q=False):
+    from starkv_b200.kernels.paged_attention import select_pages
+    dev = cuda()
+    g = torch.Generator(device=dev).manual_seed(seed)
+    n, per = len(lens), max(1, -(-max(lens) // bs))
+    bt = table(n, per, seed)
+    a, c = (torch.randn(n * per + 1, Hkv, D, generator=g, device=dev) for _ in range(2))
+    if levels:    # few distinct values: many equal scores
+        a, c = (a * levels).round() / levels, (c * levels).round() / levels
+    bounds = torch.stack([torch.minimum(a, c), torch.maximum(a, c)], 2).to(dtype)
+    q = torch.randn(n, H, D, generator=g, device=dev).to(dtype)
+    if levels:
+        q = (q * levels).round() / levels
+    if zero_q:
+        q.zero_()
+    sl = torch.tensor(lens, dtype=torch.int32, device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    got = select_pages(q, bounds, bt, sl, max(max(lens), 1), bs, top, sinks=sinks, recent=recent, status=status)
+    assert int(status) == 0
+    assert torch.equal(got.cpu(), expected(q, bounds, bt, lens, bs, top, sinks, recent))
+
+
+LENS = [0, 1, 16, 17, 127, 128, 129, 145, 1000, 5000]
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 128), (torch.bfloat16, 64)])
+@pytest.mark.parametrize("H,Hkv", [(4, 4), (8, 2), (5, 1)])
+def test_selection_at_edge_lengths(H, Hkv, dtype, D):
+    run(LENS, H, Hkv, D=D, dtype=dtype, seed=H)
+
+
+@pytest.mark.parametrize("top,sinks,recent", [(1, 0, 0), (1, 0, 1), (2, 1, 1), (9, 4, 3), (33, 0, 0), (300, 1, 1)])
+def test_kept_pages(top, sinks, recent):
+    run(LENS, 8, 2, top=top, sinks=sinks, recent=recent, seed=top)
+
+
+@pytest.mark.parametrize("bs", [1, 5, 16, 64])
+def test_block_sizes(bs):
+    run([3 * bs, 40 * bs + 1, 333], 4, 2, bs=bs, seed=bs)
+
+
+def test_long_sequences_over_a_cluster():
+    run([131071], 8, 2, top=64, seed=1)
+    run([70000, 12, 30000], 4, 1, top=129, seed=2)
+
+
+def test_ties_go_to_the_lowest_page():
+    run([16 * 700], 4, 2, top=50, levels=1, D=64, seed=3)
+    run([16 * 5000, 16 * 300], 4, 1, top=77, zero_q=True, seed=4)     # all scores equal
+    run([16 * 700] * 40, 4, 4, top=10, levels=1, D=64, seed=5)
+
+
+def test_nan_bounds_rank_first():
+    from starkv_b200.kernels.paged_attention import select_pages
+    dev = cuda()
+    bounds = torch.randn(101, 1, 2, 128, device=dev).sort(2).values.to(torch.bfloat16)
+    bt = torch.arange(1, 101, device=dev, dtype=torch.int32)[None]
+    bounds[41, 0, 0, 5] = float("nan")
+    bounds[73, 0, 1, 9] = -float("nan")
+    q = torch.randn(1, 2, 128, device=dev).to(torch.bfloat16)
+    got = select_pages(q, bounds, bt, torch.tensor([1600], dtype=torch.int32, device=dev), 1600, 16, 2, sinks=0,
+                       recent=0)
+    assert got.tolist() == [[[40, 72]]]
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("bs", [1, 5, 16, 64])
+@pytest.mark.parametrize("order", ["head", "token"])
+def test_bounds(dtype, D, bs, order):
+    from starkv_b200.kernels.paged_attention import empty_bounds, update_page_bounds
+    dev = cuda()
+    g = torch.Generator(device=dev).manual_seed(bs)
+    lens = torch.tensor([0, 1, bs, bs + 1, 5 * bs - 1, 200])
+    Hkv, n = 3, len(lens)
+    per = -(-int(lens.max()) // bs)
+    bt = table(n, per, 3)
+    shape = (n * per + 1, Hkv, bs, D)
+    k = torch.randn(shape, generator=g, device=dev).to(dtype)
+    k = k.transpose(1, 2) if order == "head" else k.transpose(1, 2).contiguous()
+    sl = lens.int().to(dev)
+    k[bt[5, 0].long(), 0, 1, 7] = float("nan")
+    k[bt[5, 1].long(), 0, 2, 3] = float("-inf")
+    for new in (1, 3, 1000, None):
+        new_lens = None if new is not None else torch.tensor([4, 0, 2, bs, 1, 150], dtype=torch.int32, device=dev)
+        bounds = empty_bounds(k)
+        bounds.fill_(9.0)
+        want = bounds.clone()
+        for b, L in enumerate(lens.tolist()):
+            fresh = min(L, new if new is not None else int(new_lens[b]))
+            for p in range((L - fresh) // bs, -(-L // bs)) if fresh else []:
+                rows = k[bt[b, p].long(), :min(bs, L - p * bs)]
+                want[bt[b, p].long(), :, 0], want[bt[b, p].long(), :, 1] = rows.amin(0), rows.amax(0)
+        update_page_bounds(k, bounds, bt, sl, int(lens.max()), max_new=new or 150, new_lens=new_lens)
+        same = torch.equal(torch.nan_to_num(bounds, nan=77.0), torch.nan_to_num(want, nan=77.0))
+        assert same, new
+
+
+def test_bounds_record_blocks_outside_the_cache():
+    from starkv_b200.kernels.paged_attention import empty_bounds, select_pages, update_page_bounds
+    dev = cuda()
+    k = torch.randn(5, 16, 1, 128, device=dev).to(torch.bfloat16)
+    bt = torch.tensor([[1, 99, 3, 4]], dtype=torch.int32, device=dev)
+    sl = torch.tensor([60], dtype=torch.int32, device=dev)
+    bounds = empty_bounds(k)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    update_page_bounds(k, bounds, bt, sl, 64, max_new=60, status=status)
+    assert int(status) == 105 and (bounds[2] == 0).all()
+    q = torch.randn(1, 1, 128, device=dev).to(torch.bfloat16)
+    status.zero_()
+    select_pages(q, bounds, bt, sl, 64, 16, 2, sinks=0, recent=0, status=status)
+    assert int(status) == 105
+
+
+def test_sparse_decode_is_the_attention_over_the_selected_pages():
+    """The whole path of a step: bounds kept page by page while a sequence grows, selection,
+    attention; with enough pages it is the full attention."""
+    import test_gpu_paged_attention as A
+    from starkv_b200.kernels.paged_attention import (empty_bounds, paged_attention_decode, sparse_paged_decode,
+                                                     update_page_bounds)
+    q, k, v, bt, sl = A.make([1000, 0, 333, 2047], 8, 2, seed=30)
+    bounds = empty_bounds(k)
+    update_page_bounds(k, bounds, bt, sl, 2047, max_new=2047)
+    out, pages = sparse_paged_decode(q, k, v, bounds, bt, sl, 2047, 0.1, 12)
+    assert torch.equal(pages.cpu(), expected(q, bounds, bt, sl.tolist(), 16, 12, 1, 1))
+    ref, _, _, tol = A.reference(q, k, v, bt, sl, 0.1, pages=pages)
+    A.check(out, ref, tol)
+    all_pages, _ = sparse_paged_decode(q, k, v, bounds, bt, sl, 2047, 0.1, 128)
+    assert torch.equal(all_pages, paged_attention_decode(q, k, v, bt, sl, 2047, 0.1))
+    # captured and replayed
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        again, _ = sparse_paged_decode(q, k, v, bounds, bt, sl, 2047, 0.1, 12)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, out)
