@@ -535,11 +535,8 @@ int starkv_kv_down_cache_write(const void* hidden, int64_t h_stride0, const void
 
 size_t starkv_paged_attention_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                               int32_t max_tokens) {
-  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
-      max_tokens <= starkv::paged_attn_tile_tokens())
-    return 0;
-  const size_t rows = std::min(16, num_heads / num_kv_heads);
-  return (size_t)2 * starkv::kPagedMaxShares * rows * (head_dim + 2) * sizeof(float);
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0) return 0;
+  return starkv::paged_attn_workspace_bytes(std::min(16, num_heads / num_kv_heads), head_dim, max_tokens);
 }
 
 int starkv_paged_attention(const StarKVPagedAttnArgs* a, void* workspace, size_t workspace_bytes, void* stream) {

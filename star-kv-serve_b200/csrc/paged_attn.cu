@@ -35,7 +35,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kSub = 16;                 // tokens of a warp's share of a tile
 constexpr int kTileTok = kWarps * kSub;  // tokens of a tile
 constexpr int kStages = 3;
-constexpr int kMaxShares = kPagedMaxShares;
+constexpr int kMaxShares = 384;          // CTAs of one call at most
 constexpr int kRowsM = 16;               // query heads of one MMA
 
 template <int D>
@@ -163,9 +163,10 @@ __device__ void find_sequence(const PagedAttnParams& p, int64_t g, int lane, int
 }
 
 // f32 partials: per share two slots (its first unit, its last one) of
-// [rows][D] outputs, then [rows] max and [rows] sum.
+// [rows][D] outputs, then [rows] max and [rows] sum, padded to whole 16-byte pieces.
+__host__ __device__ constexpr int part_floats(int rows, int D) { return rows * D + ((2 * rows + 3) & ~3); }
 __device__ __forceinline__ float* part_slot(const PagedAttnParams& p, int D, int share, int which) {
-  return p.part + (int64_t)(2 * share + which) * p.part_rows * (D + 2);
+  return p.part + (int64_t)(2 * share + which) * part_floats(p.part_rows, D);
 }
 
 template <typename T>
@@ -615,7 +616,10 @@ int launch_typed(const PagedAttnParams& p, int num_sms, cudaStream_t stream) {
 
 }  // namespace
 
-int paged_attn_tile_tokens() { return kTileTok; }
+size_t paged_attn_workspace_bytes(int rows, int head_dim, int max_tokens) {
+  if (max_tokens <= kTileTok) return 0;   // no unit has two tiles
+  return (size_t)2 * kMaxShares * part_floats(rows, head_dim) * sizeof(float);
+}
 
 int launch_paged_attn(const PagedAttnParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream) {
   if (dtype == STARKV_BF16)

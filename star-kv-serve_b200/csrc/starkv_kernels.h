@@ -150,10 +150,9 @@ struct PagedAttnParams {
   float scale;
   void* out; int64_t o_s0, o_s1;
   float* m_out; float* l_out;                        // set: the partial form (out f32, not divided)
-  float* part; int part_rows;                        // f32 [2 * shares][part_rows * (D + 2)]
+  float* part; int part_rows;                        // f32 partials (paged_attn_workspace_bytes)
   int32_t* status;
 };
-constexpr int kPagedMaxShares = 384;                 // CTAs of one call at most
 
 struct PageBoundsParams {
   const void* k; int64_t k_s0, k_s1, k_s2;
@@ -220,7 +219,7 @@ int kv_down_ctl_offset(int n_tile, int stages);
 int kv_down_split();
 int launch_kv_down_write(const CUtensorMap& tm_w, const CUtensorMap& tm_x, const DownWriteParams& p,
                          cudaStream_t stream);
-int paged_attn_tile_tokens();
+size_t paged_attn_workspace_bytes(int rows, int head_dim, int max_tokens);
 int launch_paged_attn(const PagedAttnParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
 int launch_page_bounds(const PageBoundsParams& p, int dtype, int head_dim, cudaStream_t stream);
 int launch_select_pages(SelectPagesParams p, int dtype, int head_dim, int num_sms, cudaStream_t stream);

@@ -124,6 +124,14 @@ def test_one_long_sequence_is_split_and_joined(dtype):
     run([40001], 8, 2, dtype=dtype, seed=1)
 
 
+@pytest.mark.parametrize("H,Hkv,lens", [(8, 8, [2500, 1300]), (5, 1, [12000, 9001]), (6, 2, [3000, 5000, 70]),
+                                        (12, 1, [9000, 9000, 9000]), (17, 1, [7000, 4000])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_shares_that_end_one_unit_and_begin_another(H, Hkv, lens, D):
+    # several tiles per share, so that both partial slots of a share are in use, for odd and even groups
+    run(lens, H, Hkv, D=D, seed=H)
+
+
 def test_many_sequences():
     # more sequences than a warp looks at in one step, most of them short
     g = torch.Generator().manual_seed(5)
