@@ -33,7 +33,7 @@ extern "C" {
 #endif
 
 /* 4: adds the full-rank paged cache's operators (starkv_paged_attention,
- * starkv_page_bounds, starkv_select_pages, starkv_norm_rope); 3: starkv_prefill_attention
+ * starkv_page_bounds, starkv_select_pages, starkv_sparse_paged_attention, starkv_norm_rope); 3: starkv_prefill_attention
  * and starkv_kv_down_cache_write; 2: starkv_fold_q takes a status word */
 #define STARKV_ABI_VERSION 4
 
@@ -333,8 +333,9 @@ STARKV_API int starkv_page_bounds(const StarKVPageBoundsArgs* args, void* stream
  * [n, num_kv_heads, top] (strides {sequence, head}). The first `sinks` and the last
  * `recent` pages of a sequence are always among them (sinks >= 0, recent >= 0,
  * sinks + recent <= top); their bounds are not read. Scores in 64 bits, ties to the
- * lowest page, a NaN score above all others. STARKV_EINVAL where the longest sequence
- * has more than about 196,000 pages.
+ * lowest page, a NaN score above all others. The workspace (16-byte aligned, may be null
+ * where its size is 0; max_tokens: min(max_seq_len, max_blocks * block_size)) is scratch
+ * of this call alone.
  */
 typedef struct StarKVSelectPagesArgs {
   const void* query;          int64_t q_stride[2];
@@ -346,7 +347,21 @@ typedef struct StarKVSelectPagesArgs {
   int32_t dtype, n, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, max_seq_len;
   int32_t top, sinks, recent;
 } StarKVSelectPagesArgs;
-STARKV_API int starkv_select_pages(const StarKVSelectPagesArgs* args, void* stream);
+STARKV_API size_t starkv_select_pages_workspace_bytes(int32_t n, int32_t num_kv_heads, int32_t max_tokens,
+                                                      int32_t block_size, int32_t top);
+STARKV_API int starkv_select_pages(const StarKVSelectPagesArgs* args, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/*
+ * starkv_select_pages, then starkv_paged_attention over the selected pages, the second
+ * launch prepared while the first runs. args->pages (int32 [n, num_kv_heads, top]) is
+ * written first; the other fields as in starkv_paged_attention (no partial form), bounds
+ * (strides bounds_stride0, bounds_stride1), sinks and recent as in starkv_select_pages;
+ * the workspace holds both calls' bytes, one after the other.
+ */
+STARKV_API int starkv_sparse_paged_attention(const StarKVPagedAttnArgs* args, const void* bounds,
+                  int64_t bounds_stride0, int64_t bounds_stride1, int32_t sinks, int32_t recent, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 /*
  * RMS norm of each query and key head (weights [head_dim], null: none), neox rotation of

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <mutex>
+#include <set>
+#include <utility>
 
 #include "starkv_common.cuh"
 #include "starkv_kernels.h"
@@ -107,6 +109,18 @@ int paged_max_len(int max_seq_len, int max_blocks, int block_size) {
 bool is_float_dtype(int d) { return d == STARKV_BF16 || d == STARKV_F16 || d == STARKV_F32; }
 
 }  // namespace
+
+int allow_smem(const void* fn, int bytes) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return STARKV_ECUDA;
+  static std::mutex guard;
+  static std::set<std::pair<const void*, int>> done;
+  std::lock_guard<std::mutex> lock(guard);
+  if (done.count({fn, dev})) return STARKV_OK;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return STARKV_ECUDA;
+  done.insert({fn, dev});
+  return STARKV_OK;
+}
 
 Workspace workspace_layout(int n, int num_heads, int num_kv_heads, int k_width, int v_rank, int max_seq_len) {
   Workspace w{};
@@ -539,8 +553,11 @@ size_t starkv_paged_attention_workspace_bytes(int32_t num_heads, int32_t num_kv_
   return starkv::paged_attn_workspace_bytes(std::min(16, num_heads / num_kv_heads), head_dim, max_tokens);
 }
 
-int starkv_paged_attention(const StarKVPagedAttnArgs* a, void* workspace, size_t workspace_bytes, void* stream) {
+// Checked arguments of starkv_paged_attention as kernel parameters. done: nothing to launch.
+static int paged_attn_params(const StarKVPagedAttnArgs* a, void* workspace, size_t workspace_bytes,
+                             starkv::PagedAttnParams& p, bool& done) {
   using namespace starkv;
+  done = false;
   if (!a) return STARKV_EINVAL;
   int st = paged_cache_check(a->dtype, a->n, a->num_kv_heads, a->head_dim, a->num_blocks, a->block_size);
   if (st) return st;
@@ -548,12 +565,13 @@ int starkv_paged_attention(const StarKVPagedAttnArgs* a, void* workspace, size_t
   if (a->num_heads <= 0 || a->num_heads % a->num_kv_heads || !max_len || !(a->scale > 0.f) ||
       !a->m_out != !a->l_out || (a->pages && a->top <= 0))
     return STARKV_EINVAL;
-  if (a->n == 0) return STARKV_OK;
+  done = a->n == 0;
+  if (done) return STARKV_OK;
   if (!a->query || !a->k_cache || !a->v_cache || !a->block_table || !a->seq_lens || !a->out) return STARKV_EINVAL;
   if (!rows16(a->query, a->q_stride, 2) || !rows16(a->k_cache, a->k_stride, 3) ||
       !rows16(a->v_cache, a->v_stride, 3) || !rows16(a->out, a->out_stride, 2))
     return STARKV_EALIGN;
-  PagedAttnParams p{};
+  p = PagedAttnParams{};
   p.q = a->query; p.q_s0 = a->q_stride[0]; p.q_s1 = a->q_stride[1];
   p.k = a->k_cache; p.k_s0 = a->k_stride[0]; p.k_s1 = a->k_stride[1]; p.k_s2 = a->k_stride[2];
   p.v = a->v_cache; p.v_s0 = a->v_stride[0]; p.v_s1 = a->v_stride[1]; p.v_s2 = a->v_stride[2];
@@ -583,8 +601,16 @@ int starkv_paged_attention(const StarKVPagedAttnArgs* a, void* workspace, size_t
   if (need && (reinterpret_cast<uintptr_t>(workspace) & 15)) return STARKV_EALIGN;
   p.part = reinterpret_cast<float*>(workspace);
   p.status = a->status;
+  return STARKV_OK;
+}
+
+int starkv_paged_attention(const StarKVPagedAttnArgs* a, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace starkv;
+  PagedAttnParams p;
+  bool done;
+  if (const int st = paged_attn_params(a, workspace, workspace_bytes, p, done); st || done) return st;
   DeviceInfo dev;
-  if ((st = device_info(dev))) return st;
+  if (const int st = device_info(dev)) return st;
   return launch_paged_attn(p, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream);
 }
 
@@ -614,8 +640,18 @@ int starkv_page_bounds(const StarKVPageBoundsArgs* a, void* stream) {
   return launch_page_bounds(p, a->dtype, a->head_dim, (cudaStream_t)stream);
 }
 
-int starkv_select_pages(const StarKVSelectPagesArgs* a, void* stream) {
+// 8 bytes of score per page of the longest sequence, (sequence and) KV head
+size_t starkv_select_pages_workspace_bytes(int32_t n, int32_t num_kv_heads, int32_t max_tokens, int32_t block_size,
+                                           int32_t top) {
+  if (n <= 0 || num_kv_heads <= 0 || max_tokens <= 0 || block_size <= 0) return 0;
+  const size_t pages = ((size_t)max_tokens + block_size - 1) / block_size;
+  return pages <= (size_t)std::max(top, 0) ? 0 : (pages * n * num_kv_heads * 8 + 255) / 256 * 256;
+}
+
+static int select_pages_params(const StarKVSelectPagesArgs* a, void* workspace, size_t workspace_bytes,
+                               starkv::SelectPagesParams& p, bool& done) {
   using namespace starkv;
+  done = false;
   if (!a) return STARKV_EINVAL;
   int st = paged_cache_check(a->dtype, a->n, a->num_kv_heads, a->head_dim, a->num_blocks, a->block_size);
   if (st) return st;
@@ -623,10 +659,11 @@ int starkv_select_pages(const StarKVSelectPagesArgs* a, void* stream) {
   if (a->num_heads <= 0 || a->num_heads % a->num_kv_heads || !max_len || a->top <= 0 || a->sinks < 0 ||
       a->recent < 0 || (int64_t)a->sinks + a->recent > a->top)
     return STARKV_EINVAL;
-  if (a->n == 0) return STARKV_OK;
+  done = a->n == 0;
+  if (done) return STARKV_OK;
   if (!a->query || !a->bounds || !a->block_table || !a->seq_lens || !a->pages) return STARKV_EINVAL;
   if (!rows16(a->query, a->q_stride, 2) || !rows16(a->bounds, a->bounds_stride, 2)) return STARKV_EALIGN;
-  SelectPagesParams p{};
+  p = SelectPagesParams{};
   p.q = a->query; p.q_s0 = a->q_stride[0]; p.q_s1 = a->q_stride[1];
   p.bounds = a->bounds; p.b_s0 = a->bounds_stride[0]; p.b_s1 = a->bounds_stride[1];
   p.block_table = a->block_table; p.bt_s0 = a->bt_stride[0]; p.bt_s1 = a->bt_stride[1];
@@ -635,9 +672,54 @@ int starkv_select_pages(const StarKVSelectPagesArgs* a, void* stream) {
   p.group = a->num_heads / a->num_kv_heads; p.top = a->top; p.sinks = a->sinks; p.recent = a->recent;
   p.pages = a->pages; p.pg_s0 = a->pages_stride[0]; p.pg_s1 = a->pages_stride[1];
   p.status = a->status;
+  const size_t need = starkv_select_pages_workspace_bytes(a->n, a->num_kv_heads, max_len, a->block_size, a->top);
+  if (need && (!workspace || workspace_bytes < need)) return STARKV_EWORKSPACE;
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 15)) return STARKV_EALIGN;
+  p.keys = reinterpret_cast<uint64_t*>(workspace);
+  p.key_stride = ((int64_t)max_len + a->block_size - 1) / a->block_size;
+  return STARKV_OK;
+}
+
+int starkv_select_pages(const StarKVSelectPagesArgs* a, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace starkv;
+  SelectPagesParams p;
+  bool done;
+  if (const int st = select_pages_params(a, workspace, workspace_bytes, p, done); st || done) return st;
   DeviceInfo dev;
-  if ((st = device_info(dev))) return st;
+  if (const int st = device_info(dev)) return st;
   return launch_select_pages(p, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream);
+}
+
+int starkv_sparse_paged_attention(const StarKVPagedAttnArgs* a, const void* bounds, int64_t bounds_stride0,
+                                  int64_t bounds_stride1, int32_t sinks, int32_t recent, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  using namespace starkv;
+  if (!a || !a->pages || a->m_out || a->l_out) return STARKV_EINVAL;
+  StarKVSelectPagesArgs s{};
+  s.query = a->query; s.q_stride[0] = a->q_stride[0]; s.q_stride[1] = a->q_stride[1];
+  s.bounds = bounds; s.bounds_stride[0] = bounds_stride0; s.bounds_stride[1] = bounds_stride1;
+  s.block_table = a->block_table; s.bt_stride[0] = a->bt_stride[0]; s.bt_stride[1] = a->bt_stride[1];
+  s.seq_lens = a->seq_lens;
+  s.pages = const_cast<int32_t*>(a->pages);
+  s.pages_stride[0] = a->pages_stride[0]; s.pages_stride[1] = a->pages_stride[1];
+  s.status = a->status; s.dtype = a->dtype; s.n = a->n; s.num_heads = a->num_heads;
+  s.num_kv_heads = a->num_kv_heads; s.head_dim = a->head_dim; s.num_blocks = a->num_blocks;
+  s.block_size = a->block_size; s.max_blocks = a->max_blocks; s.max_seq_len = a->max_seq_len;
+  s.top = a->top; s.sinks = sinks; s.recent = recent;
+  SelectPagesParams sp;
+  PagedAttnParams ap;
+  bool done;
+  if (const int st = select_pages_params(&s, workspace, workspace_bytes, sp, done); st || done) return st;
+  const size_t used = starkv_select_pages_workspace_bytes(a->n, a->num_kv_heads, sp.max_len, a->block_size, a->top);
+  if (const int st = paged_attn_params(a, workspace ? static_cast<uint8_t*>(workspace) + used : nullptr,
+                                       workspace_bytes > used ? workspace_bytes - used : 0, ap, done);
+      st || done)
+    return st;
+  DeviceInfo dev;
+  if (const int st = device_info(dev)) return st;
+  if (const int st = launch_select_pages(sp, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream)) return st;
+  ap.after_select = 1;
+  return launch_paged_attn(ap, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream);
 }
 
 int starkv_norm_rope(const StarKVNormRopeArgs* a, void* stream) {

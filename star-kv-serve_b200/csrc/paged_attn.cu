@@ -5,7 +5,7 @@
 //
 // What bounds it: every K and V row is read once and used for G heads, 4 G FLOP per
 // element of 2 bytes, so the cache read is the cost. The tokens of all (sequence, KV
-// head) units are laid end to end in 64-token tiles and every CTA of one wave takes an
+// head) units are laid end to end in items of 64 tokens and every CTA of one wave takes an
 // equal run of them, whatever the mix of lengths. A unit that lies inside one CTA's run
 // is finished there; a unit that crosses CTA borders leaves one partial (max, sum,
 // unnormalised output) per CTA, and join_kernel adds them in the order of the CTAs, so
@@ -21,8 +21,10 @@
 // sums. P is split into a high and a low part of the cache's type, so that its rounding
 // (2^-9 for bf16) does not show in the result; with G <= 8 both parts share one MMA (rows
 // 0-7 and 8-15), so the split costs nothing.
+#include <algorithm>
 #include <type_traits>
 
+#include "flat_items.cuh"
 #include "starkv_common.cuh"
 #include "starkv_kernels.h"
 
@@ -34,6 +36,8 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kSub = 16;                 // tokens of a warp's share of a tile
 constexpr int kTileTok = kWarps * kSub;  // tokens of a tile
+constexpr int kTileShift = 6, kWholeShift = 8;
+constexpr int kWholeTokens = 1 << kWholeShift;   // units of at most this many tokens are not split
 constexpr int kStages = 3;
 constexpr int kMaxShares = 384;          // CTAs of one call at most
 constexpr int kRowsM = 16;               // query heads of one MMA
@@ -124,42 +128,9 @@ __device__ __forceinline__ int unit_tokens(const PagedAttnParams& p, int b) {
   if (!p.pages) return L;
   return min(p.top, (L + p.block_size - 1) / p.block_size) * p.block_size;
 }
-__device__ __forceinline__ int unit_tiles(const PagedAttnParams& p, int b) {
-  return b < p.n ? (unit_tokens(p, b) + kTileTok - 1) / kTileTok : 0;
-}
-
-// Total tiles (of one unit per sequence) of the batch; every warp computes it.
-__device__ int64_t total_tiles(const PagedAttnParams& p, int lane) {
-  int64_t s = 0;
-  for (int b = lane; b < p.n; b += 32) s += unit_tiles(p, b);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-  return s;
-}
-
-// The sequence that holds global tile g (tiles of `units` units each, sequences in
-// order) and the global index of its first tile. Every warp computes it.
-__device__ void find_sequence(const PagedAttnParams& p, int64_t g, int lane, int& seq, int64_t& first) {
-  int64_t base = 0;
-  for (int b0 = 0; b0 < p.n; b0 += 32) {
-    const int64_t mine = (int64_t)unit_tiles(p, b0 + lane) * p.units;
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(~0u, incl, o);
-      if (lane >= o) incl += v;
-    }
-    const uint32_t hit = __ballot_sync(~0u, base + incl > g);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      seq = b0 + l;
-      first = base + __shfl_sync(~0u, incl - mine, l);
-      return;
-    }
-    base += __shfl_sync(~0u, incl, 31);
-  }
-  seq = p.n;
-  first = base;
+// Work items (runs of 2^item_shift tokens) of a unit of sequence b.
+__device__ __forceinline__ int unit_items(const PagedAttnParams& p, int b) {
+  return b < p.n ? (unit_tokens(p, b) + (1 << p.item_shift) - 1) >> p.item_shift : 0;
 }
 
 // f32 partials: per share two slots (its first unit, its last one) of
@@ -196,8 +167,9 @@ __device__ __forceinline__ void store_out(const PagedAttnParams& p, int b, int h
   store4(reinterpret_cast<T*>(p.out) + at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
-// kTwo: more than 8 query heads in the unit's MMA rows.
-template <typename T, int D, bool kTwo, bool kSparse>
+// kTwo: more than 8 query heads in the unit's MMA rows. kThird: weights in three parts,
+// for the bf16 partial form, whose output is f32.
+template <typename T, int D, bool kTwo, bool kSparse, bool kThird>
 __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttnParams p) {
   using R = Ring<D>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -211,6 +183,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   const float c_log2 = p.scale * 1.4426950408889634f;
   constexpr float kBias = weight_bias<T>();
 
+  // the joining kernel's blocks may take the place of CTAs that are done; they wait for all
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // sequences without a token have no tile: their outputs are written here
   for (int b = blockIdx.x; b < p.n; b += gridDim.x) {
     if (unit_tokens(p, b) > 0) continue;
@@ -218,19 +192,20 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
       store_out<T>(p, b, i / (D / 4), (i % (D / 4)) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
   }
 
-  const int64_t total = total_tiles(p, lane) * p.units;
-  const int shares = (int)min((int64_t)gridDim.x, total);
+  const auto count = [&](int b) { return unit_items(p, b) * p.units; };
+  FlatItems<decltype(count)> all(count, p.n, lane);
+  const int shares = min((int)gridDim.x, all.total);
+  if (kSparse && p.after_select) asm volatile("griddepcontrol.wait;" ::: "memory");   // the lists are written
   if ((int)blockIdx.x >= shares) return;
-  const int64_t g0 = total * blockIdx.x / shares, g1 = total * (blockIdx.x + 1) / shares;
-  int b;
-  int64_t first;
-  find_sequence(p, g0, lane, b, first);
-  int tiles = unit_tiles(p, b);
-  int unit = (int)((g0 - first) / tiles);
-  int t0 = (int)((g0 - first) % tiles);
+  const int g0 = share_begin(all.total, blockIdx.x, shares), g1 = share_begin(all.total, blockIdx.x + 1, shares);
+  int b, first;
+  all.place(g0, b, first);
+  int items = unit_items(p, b);
+  int unit = (g0 - first) / items;
+  int t0 = (g0 - first) % items;
 
-  for (int64_t g = g0; g < g1;) {
-    const int t1 = (int)min((int64_t)tiles, t0 + (g1 - g));
+  for (int g = g0; g < g1;) {
+    const int t1 = min(items, t0 + (g1 - g));
     const int hk = unit / p.head_groups, hg = unit % p.head_groups;
     const int head0 = hk * p.group + hg * kRowsM;
     const int rows = min(kRowsM, p.group - hg * kRowsM);
@@ -241,9 +216,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
     const char* kbase = reinterpret_cast<const char*>(p.k) + hk * p.k_s2 * 2;
     const char* vbase = reinterpret_cast<const char*>(p.v) + hk * p.v_s2 * 2;
     // this warp's 16-token subtiles of the segment
-    int subs = t1 - t0;
-    if (subs && (t1 - 1) * kTileTok + warp * kSub >= tokens) --subs;
-    const int base0 = t0 * kTileTok + warp * kSub;
+    const int base0 = (t0 << p.item_shift) + warp * kSub;
+    const int end = (int)min((int64_t)t1 << p.item_shift, (int64_t)tokens);
+    const int subs = max(end - base0 + kTileTok - 1, 0) / kTileTok;
 
     // Q as A fragments
     uint32_t qa[kKSteps][4];
@@ -402,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
       const float p00 = ex2(fmaf(s0[0] - u0, c_log2, kBias)), p01 = ex2(fmaf(s0[1] - u0, c_log2, kBias));
       const float p02 = ex2(fmaf(s1[0] - u0, c_log2, kBias)), p03 = ex2(fmaf(s1[1] - u0, c_log2, kBias));
       l0 += (p00 + p01) + (p02 + p03);
-      uint32_t pa[4], pl[4];
+      uint32_t pa[4], pl[4], t1a = 0, t3a = 0;
       pa[0] = pack2(T{}, p00, p01);
       pa[2] = pack2(T{}, p02, p03);
       const float2 h0 = unpack2(T{}, pa[0]), h2 = unpack2(T{}, pa[2]);
@@ -417,9 +392,25 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
         const float2 h1 = unpack2(T{}, pa[1]), h3 = unpack2(T{}, pa[3]);
         pl[1] = pack2(T{}, p10 - h1.x, p11 - h1.y);
         pl[3] = pack2(T{}, p12 - h3.x, p13 - h3.y);
+        if (kThird) {
+          const float2 e1 = unpack2(T{}, pl[1]), e3 = unpack2(T{}, pl[3]);
+          t1a = pack2(T{}, p10 - h1.x - e1.x, p11 - h1.y - e1.y);
+          t3a = pack2(T{}, p12 - h3.x - e3.x, p13 - h3.y - e3.y);
+        }
       } else {
         pa[1] = pl[0];
         pa[3] = pl[2];
+      }
+      uint32_t pt[4] = {0u, 0u, 0u, 0u};
+      if (kThird) {
+        // f32 output: what the two parts leave (2^-16) goes into a third
+        const float2 e0 = unpack2(T{}, pl[0]), e2 = unpack2(T{}, pl[2]);
+        pt[0] = pack2(T{}, p00 - h0.x - e0.x, p01 - h0.y - e0.y);
+        pt[2] = pack2(T{}, p02 - h2.x - e2.x, p03 - h2.y - e2.y);
+        if (kTwo) {
+          pt[1] = t1a;
+          pt[3] = t3a;
+        }
       }
       // ---- O += P V ----
       {
@@ -435,10 +426,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
             mma16816<T>(o[2 * j], pl, r[0], r[1]);
             mma16816<T>(o[2 * j + 1], pl, r[2], r[3]);
           }
+          if (kThird) {
+            mma16816<T>(o[2 * j], pt, r[0], r[1]);
+            mma16816<T>(o[2 * j + 1], pt, r[2], r[3]);
+          }
         }
       }
     }
-    if (g + (t1 - t0) >= g1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     cp_wait<0>();
     __syncthreads();   // no copy in flight, no warp reads its ring: the space holds the warps' outputs now
 
@@ -467,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
             make_float2(o[j][2], o[j][3]);
     }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
+    const bool whole = t0 == 0 && t1 == items;
     float* part = whole ? nullptr : part_slot(p, D, blockIdx.x, g > g0);
     for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
       const int row = i / (D / 4), c = (i % (D / 4)) * 4;
@@ -503,112 +497,157 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
     t0 = 0;
     if (g < g1 && ++unit == p.units) {
       unit = 0;
-      do tiles = unit_tiles(p, ++b);
-      while (tiles == 0 && b < p.n);
+      do items = unit_items(p, ++b);
+      while (items == 0 && b < p.n);
       if (b >= p.n) break;   // not reached: g < g1 <= total
     }
   }
 }
 
-// Adds the partials of the units that cross a border between shares. Block (i, row): if
-// the border after share i lies inside a unit, and share i is the unit's first, the
-// unit's shares i .. j are added, row by row; kLanes groups of threads take every
-// kLanes-th share, and their sums are added in order.
+// Adds the partials of the units that cross a border between shares. Block i: if the
+// border after share i lies inside a unit, and share i is the unit's first, the unit's
+// shares i .. j are added. A thread takes four channels of a row; the groups of
+// rows * D / 4 threads take every kLanes-th share, four at a time in flight, and the
+// groups' sums are added in order.
+constexpr int kJoinThreads = 512;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) join_kernel(const PagedAttnParams p, int grid) {
-  constexpr int kCols = D / 4, kLanes = 256 / kCols;
-  __shared__ float sm[kLanes], sl[kLanes];
-  __shared__ float4 so[kLanes][kCols];
-  const int lane = threadIdx.x & 31;
-  const int64_t total = total_tiles(p, lane) * p.units;
-  const int shares = (int)min((int64_t)grid, total);
-  const int i0 = blockIdx.x, row = blockIdx.y;
-  int64_t u0 = 0, u1 = 0;
-  int b = 0, hk = 0, hg = 0;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttnParams p, int grid) {
+  constexpr int kCols = D / 4;
+  constexpr int kAhead = 4;
+  __shared__ float4 so[kJoinThreads];
+  __shared__ float2 sml[kJoinThreads];
+  const int width = p.part_rows * kCols, lanes = kJoinThreads / width;   // part_rows <= 16: width <= 512
+  const auto count = [&](int b) { return unit_items(p, b) * p.units; };
+  FlatItems<decltype(count)> all(count, p.n, threadIdx.x & 31);
+  const int total = all.total;
+  const int shares = min(grid, total);
+  const int i0 = blockIdx.x;
+  int u0 = 0, u1 = 0, b = 0, hk = 0, hg = 0;
   bool mine = false;
   if (i0 + 1 < shares) {
-    const int64_t border = total * (i0 + 1) / shares;   // first tile of share i0 + 1
-    int64_t first;
-    find_sequence(p, border, lane, b, first);
-    const int tiles = unit_tiles(p, b);
-    const int unit = (int)((border - first) / tiles);
-    u0 = first + (int64_t)unit * tiles;
-    u1 = u0 + tiles;
+    const int border = share_begin(total, i0 + 1, shares);
+    int first;
+    all.place(border, b, first);
+    const int items = unit_items(p, b);
+    const int unit = (border - first) / items;
+    u0 = first + unit * items;
+    u1 = u0 + items;
     hk = unit / p.head_groups;
     hg = unit % p.head_groups;
-    mine = u0 < border && total * i0 / shares <= u0 && row < min(kRowsM, p.group - hg * kRowsM);
+    mine = u0 < border && share_begin(total, i0, shares) <= u0;
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the partials are written
   if (!mine) return;
-  // share of the unit's last tile: the largest i with floor(total i / shares) <= u1 - 1
-  const int i1 = (int)((u1 * shares + total - 1) / total) - 1;
-  const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+  // share of the unit's last item: the largest i with share_begin(i) <= u1 - 1
+  const int i1 = (int)(((int64_t)u1 * shares + total - 1) / total) - 1;
+  const int late = share_begin(total, i0, shares) < u0;   // the unit is not the first of share i0
+  const int col = threadIdx.x % kCols, row = threadIdx.x / kCols % p.part_rows, grp = threadIdx.x / width;
+  const bool in = grp < lanes && row < min(kRowsM, p.group - hg * kRowsM);
   const float c_log2 = p.scale * 1.4426950408889634f;
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = i0 + grp; i <= i1; i += kLanes) {
-    const float* part = part_slot(p, D, i, i == i0 && total * i0 / shares < u0);
-    const float pm = part[p.part_rows * D + row], pl = part[p.part_rows * (D + 1) + row];
-    const float4 v = *reinterpret_cast<const float4*>(part + row * D + col * 4);
-    const float nm = fmaxf(m, pm);
-    const float fa = m == nm ? 1.f : ex2((m - nm) * c_log2), fb = pm == nm ? 1.f : ex2((pm - nm) * c_log2);
-    acc.x = acc.x * fa + v.x * fb;
-    acc.y = acc.y * fa + v.y * fb;
-    acc.z = acc.z * fa + v.z * fb;
-    acc.w = acc.w * fa + v.w * fb;
-    l = l * fa + pl * fb;
+  for (int ib = in ? i0 + grp : i1 + 1; ib <= i1; ib += lanes * kAhead) {
+    float pm[kAhead], pl[kAhead];
+    float4 v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = ib + u * lanes;
+      pm[u] = -INFINITY;
+      pl[u] = 0.f;
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i <= i1) {
+        const float* part = part_slot(p, D, i, i == i0 && late);
+        pm[u] = part[p.part_rows * D + row];
+        pl[u] = part[p.part_rows * (D + 1) + row];
+        v[u] = *reinterpret_cast<const float4*>(part + row * D + col * 4);
+      }
+    }
+    float nm = m;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) nm = fmaxf(nm, pm[u]);
+    const float fa = m == nm ? 1.f : ex2((m - nm) * c_log2);
+    acc.x *= fa;
+    acc.y *= fa;
+    acc.z *= fa;
+    acc.w *= fa;
+    l *= fa;
     m = nm;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float f = pm[u] == m ? 1.f : ex2((pm[u] - m) * c_log2);
+      acc.x += f * v[u].x;
+      acc.y += f * v[u].y;
+      acc.z += f * v[u].z;
+      acc.w += f * v[u].w;
+      l += f * pl[u];
+    }
   }
-  so[grp][col] = acc;
-  if (col == 0) {
-    sm[grp] = m;
-    sl[grp] = l;
-  }
+  so[threadIdx.x] = acc;
+  sml[threadIdx.x] = make_float2(m, l);
   __syncthreads();
-  if (grp) return;
-  float M = -INFINITY;
-  for (int w = 0; w < kLanes; ++w) M = fmaxf(M, sm[w]);
+  if (grp || !in) return;
+  float M = m;
+  for (int w = 1; w < lanes; ++w) M = fmaxf(M, sml[threadIdx.x + w * width].x);
   acc = make_float4(0.f, 0.f, 0.f, 0.f);
   l = 0.f;
-  for (int w = 0; w < kLanes; ++w) {
-    const float f = sm[w] == M ? 1.f : ex2((sm[w] - M) * c_log2);
-    acc.x += f * so[w][col].x;
-    acc.y += f * so[w][col].y;
-    acc.z += f * so[w][col].z;
-    acc.w += f * so[w][col].w;
-    l += f * sl[w];
+  for (int w = 0; w < lanes; ++w) {
+    const float2 ml = sml[threadIdx.x + w * width];
+    const float4 v = so[threadIdx.x + w * width];
+    const float f = ml.x == M ? 1.f : ex2((ml.x - M) * c_log2);
+    acc.x += f * v.x;
+    acc.y += f * v.y;
+    acc.z += f * v.z;
+    acc.w += f * v.w;
+    l += f * ml.y;
   }
   store_out<T>(p, b, hk * p.group + hg * kRowsM + row, col * 4, acc, M, l);
+}
+
+template <typename T, int D, bool kSparse>
+const void* attn_fn(bool two, bool third) {
+  constexpr bool k3 = std::is_same<T, __nv_bfloat16>::value;
+  if (third)
+    return two ? (const void*)paged_attn_kernel<T, D, true, kSparse, k3>
+               : (const void*)paged_attn_kernel<T, D, false, kSparse, k3>;
+  return two ? (const void*)paged_attn_kernel<T, D, true, kSparse, false>
+             : (const void*)paged_attn_kernel<T, D, false, kSparse, false>;
 }
 
 template <typename T, int D>
 int launch_typed(const PagedAttnParams& p, int num_sms, cudaStream_t stream) {
   const bool two = p.group > 8;
-  const void* fn = p.pages ? (two ? (const void*)paged_attn_kernel<T, D, true, true>
-                                  : (const void*)paged_attn_kernel<T, D, false, true>)
-                           : (two ? (const void*)paged_attn_kernel<T, D, true, false>
-                                  : (const void*)paged_attn_kernel<T, D, false, false>);
+  // f16 parts hold 22 bits, as much as f32 sums need
+  const bool third = p.m_out && std::is_same<T, __nv_bfloat16>::value;
+  const void* fn = p.pages ? attn_fn<T, D, true>(two, third) : attn_fn<T, D, false>(two, third);
   const int smem = Ring<D>::bytes;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return STARKV_ECUDA;
-  const int64_t most = (int64_t)p.n * p.units * ((p.max_unit_tokens + kTileTok - 1) / kTileTok);
-  int64_t grid = 2 * num_sms;
-  if (grid > kMaxShares) grid = kMaxShares;
-  if (grid > most) grid = most;
-  if (grid < 1) grid = 1;
+  if (const int st = allow_smem(fn, smem)) return st;
   PagedAttnParams q = p;
-  void* args[] = {&q};
-  if (cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), args, smem, stream) != cudaSuccess) return STARKV_ECUDA;
-  if (grid == 1 || p.max_unit_tokens <= kTileTok) return STARKV_OK;   // no unit has two tiles in two shares
+  q.item_shift = p.max_unit_tokens <= kWholeTokens ? kWholeShift : kTileShift;
+  const auto most = [&] {
+    return (int64_t)p.n * p.units * ((p.max_unit_tokens + ((int64_t)1 << q.item_shift) - 1) >> q.item_shift);
+  };
+  while (most() > 0x7fffffff && q.item_shift < 30) ++q.item_shift;   // 32-bit item numbers
+  if (most() > 0x7fffffff) return STARKV_EINVAL;
+  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>({2 * num_sms, kMaxShares, most()}));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)grid - 1, p.part_rows);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
+  cfg.numAttrs = p.after_select;   // behind pick_kernel alone may the launch come early
+  void* args[] = {&q};
+  if (cudaLaunchKernelExC(&cfg, fn, args) != cudaSuccess) return STARKV_ECUDA;
+  if (grid == 1 || p.max_unit_tokens <= kWholeTokens) return STARKV_OK;   // no unit is in two shares
+  cfg.gridDim = dim3((unsigned)grid - 1);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  int g = (int)grid;
+  int g = grid;
   void* jargs[] = {&q, &g};
   if (cudaLaunchKernelExC(&cfg, (const void*)join_kernel<T, D>, jargs) != cudaSuccess) return STARKV_ECUDA;
   return STARKV_OK;
@@ -617,7 +656,7 @@ int launch_typed(const PagedAttnParams& p, int num_sms, cudaStream_t stream) {
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int rows, int head_dim, int max_tokens) {
-  if (max_tokens <= kTileTok) return 0;   // no unit has two tiles
+  if (max_tokens <= kWholeTokens) return 0;   // every unit is one item
   return (size_t)2 * kMaxShares * part_floats(rows, head_dim) * sizeof(float);
 }
 

@@ -4,7 +4,7 @@
 // channel. It reads each key once and writes 2 D values per page; the read is the cost.
 // A warp takes one (page, head), 16 bytes per lane, whole rows at a time.
 //
-// select_kernel: for each (sequence, KV head) the `top` pages of the highest score
+// Selection: for each (sequence, KV head) the `top` pages of the highest score
 //   score(page) = sum_{g in group} sum_d max(q[g, d] lo[d], q[g, d] hi[d])
 //               = sum_d up[d] hi[d] + down[d] lo[d],
 //   up = sum_g max(q[g], 0),  down = sum_g min(q[g], 0),
@@ -14,13 +14,15 @@
 // pages next to the border does not depend on how the sum was split (32-bit sums put
 // about one of a thousand selections on the other side).
 //
-// A cluster of CTAs takes one (sequence, KV head), each CTA a run of pages whose scores
-// stay in its shared memory as order-preserving 64-bit keys; the border is found by
-// radix selection from the highest bit in which the keys differ, the histograms added
-// through distributed shared memory. Ties go to the lowest page index.
-#include <cooperative_groups.h>
+// score_kernel takes the batch's pages in runs of 32, an equal number of runs per warp
+// whatever the mix of lengths, and writes order-preserving 64-bit keys. pick_kernel takes
+// a CTA per (sequence, KV head) and finds the border by radix selection from the highest
+// bit in which the unit's keys differ (one or two passes of 8 bits on real scores). Ties
+// go to the lowest page.
+#include <algorithm>
 #include <type_traits>
 
+#include "flat_items.cuh"
 #include "starkv_common.cuh"
 #include "starkv_kernels.h"
 
@@ -28,12 +30,8 @@ namespace starkv {
 
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxCluster = 8;
-constexpr size_t kKeyBytes = 192 * 1024;
 
 __device__ __forceinline__ uint32_t min2(__nv_bfloat16, uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
@@ -119,100 +117,168 @@ __device__ __forceinline__ uint64_t order_key(double x) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) select_kernel(const SelectPagesParams p) {
-  extern __shared__ __align__(16) uint64_t keys[];
-  __shared__ uint32_t hist[2][256];
-  __shared__ uint64_t range[2];                      // smallest, largest key of this CTA
-  __shared__ uint64_t warp_lo[kWarps], warp_hi[kWarps];
-  __shared__ uint32_t scan[kWarps], found[3];        // bin, still needed in it, its count
-  __shared__ int n_gt[kWarps], n_eq[kWarps], cta_counts[2], before[2];
-  constexpr int LP = 2 * D / 8;                      // lanes of one page's bounds
-  constexpr int kPer = 8 * (32 / LP);                // pages of a warp's step
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t unit = blockIdx.x / C;
-  const int hk = (int)(unit % p.num_kv_heads), b = (int)(unit / p.num_kv_heads);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// Pages of sequence b, and how many of them compete: all but the kept ones, none where
+// every page is taken.
+__device__ __forceinline__ int pages_of(const SelectPagesParams& p, int b) {
   const int L = min(max(p.seq_lens[b], 0), p.max_len);
-  const int P = (int)(((int64_t)L + p.block_size - 1) / p.block_size);
-  int32_t* out = p.pages + b * p.pg_s0 + hk * p.pg_s1;
-  if (P <= p.top) {   // every page, then -1
-    if (rank == 0)
-      for (int i = tid; i < p.top; i += kThreads) out[i] = i < P ? i : -1;
-    return;
-  }
-  const int need = p.top - p.sinks - p.recent;       // >= 0; P > top: the kept pages do not overlap
-  if (rank == 0) {
-    for (int i = tid; i < p.sinks; i += kThreads) out[i] = i;
-    for (int i = tid; i < p.recent; i += kThreads) out[p.top - p.recent + i] = P - p.recent + i;
-  }
-  if (need == 0) return;
-  const int N = P - p.sinks - p.recent;              // pages that compete, > need
-  const int c0 = (int)((int64_t)N * rank / C), cnt = (int)((int64_t)N * (rank + 1) / C) - c0;
+  return (int)(((int64_t)L + p.block_size - 1) / p.block_size);
+}
+__device__ __forceinline__ int competing(const SelectPagesParams& p, int pages) {
+  return pages <= p.top || p.sinks + p.recent == p.top ? 0 : pages - p.sinks - p.recent;
+}
 
-  // ---- scores of this CTA's pages ----
-  uint64_t k_lo = ~0ull, k_hi = 0;
-  {
-    const int e = lane % LP, sub = lane / LP;
-    const int d = (e * 8) % D;
-    const bool upper = e * 8 >= D;
-    double w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 0.0;
-    for (int g = 0; g < p.group; ++g) {
-      const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group + g) * p.q_s1 + d;
-      float f[8];
-      to_f32x8(T{}, *reinterpret_cast<const uint4*>(q), f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] += (double)(upper ? (f[i] < 0.f ? 0.f : f[i]) : (f[i] > 0.f ? 0.f : f[i]));
-    }
-    const int32_t* bt = p.block_table + b * p.bt_s0;
+constexpr int kRun = 32;     // pages of a run
+constexpr int kStep = 4;     // pages of a lane's step
+constexpr int kRing = 3;     // steps in the copies' ring
+constexpr int kRingBytes = kRing * kStep * 16 * kThreads;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesParams p) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  constexpr int LP = 2 * D / 8;                      // lanes of one page's bounds
+  constexpr int kPer = kStep * (32 / LP);            // pages of a warp's step
+  constexpr int kSteps = kRun / kPer;                // steps of a run
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int e = lane % LP, sub = lane / LP;
+  const int d = (e * 8) % D;
+  const bool upper = e * 8 >= D;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // pick_kernel waits for all of this one
+  const auto count = [&](int b) { return (competing(p, pages_of(p, b)) + kRun - 1) / kRun * p.num_kv_heads; };
+  FlatItems<decltype(count)> all(count, p.n, lane);
+  const int shares = min((int)gridDim.x * kWarps, all.total);
+  const int share = blockIdx.x + warp * gridDim.x;   // a warp of every CTA before the second of one
+  if (share >= shares) return;
+  const int g1 = share_begin(all.total, share + 1, shares);
+  int g = share_begin(all.total, share, shares);
+  int b, first;
+  all.place(g, b, first);
+  int N = competing(p, pages_of(p, b)), runs = (N + kRun - 1) / kRun;
+  int hk = (g - first) / runs, run = (g - first) % runs;
+
+  while (g < g1) {
+    // the share's runs of this (sequence, KV head)
+    const int here = min(runs - run, g1 - g);
+    const int i0 = run * kRun, i1 = min(i0 + here * kRun, N);   // competing pages i0 .. i1 - 1
+    const int steps = (i1 - i0 + kPer - 1) / kPer;
+    const int32_t* bt = p.block_table + b * p.bt_s0 + (int64_t)p.sinks * p.bt_s1;
     const T* bounds = reinterpret_cast<const T*>(p.bounds) + (int64_t)hk * p.b_s1 + e * 8;
-    auto block_of = [&](int i0) {   // lanes 0 .. kPer-1: the blocks of pages i0 .. i0 + kPer - 1
-      const int i = i0 + lane;
-      if (lane >= kPer || i >= cnt) return 0;
-      int blk = bt[(int64_t)(p.sinks + c0 + i) * p.bt_s1];
+    // A lane copies its own 16 bytes of a page into its own slots of the ring (cp.async,
+    // two steps ahead): no barrier between copy and use. Block ids come 32 at a time.
+    const uint32_t slots = smem_u32(ring) + tid * 16;
+    auto blocks_from = [&](int i) {   // lane l: the block of competing page i + l
+      if (i + lane >= i1) return 0;
+      int blk = bt[(int64_t)(i + lane) * p.bt_s1];
       if ((unsigned)blk >= (unsigned)p.num_blocks) {
         record_status(p.status, STARKV_EBOUNDS);
         blk = 0;
       }
       return blk;
     };
-    int nxt = block_of(warp * kPer);
-    for (int i0 = warp * kPer; i0 < cnt; i0 += kWarps * kPer) {
-      const int cur = nxt;
-      uint4 v[8];
+    int cur = 0, nxt = blocks_from(i0);
+    auto issue = [&](int j) {
+      if (j % kSteps == 0) {
+        cur = nxt;
+        nxt = blocks_from(i0 + (j / kSteps + 1) * kRun);
+      }
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        v[u] = *reinterpret_cast<const uint4*>(bounds + (int64_t)__shfl_sync(~0u, cur, sub * 8 + u) * p.b_s0);
-      nxt = block_of(i0 + kWarps * kPer);
-      double s[8];
+      for (int u = 0; u < kStep; ++u) {
+        const int blk = __shfl_sync(~0u, cur, j % kSteps * kPer + sub * kStep + u);   // a page past the end: block 0
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + (j % kRing * kStep + u) * kThreads * 16),
+                     "l"(bounds + (int64_t)blk * p.b_s0)
+                     : "memory");
+      }
+    };
+    issue(0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (steps > 1) issue(1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    double w[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+    for (int i = 0; i < 8; ++i) w[i] = 0.0;
+    const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group) * p.q_s1 + d;
+#pragma unroll 4
+    for (int h = 0; h < p.group; ++h) {
+      float f[8];
+      to_f32x8(T{}, *reinterpret_cast<const uint4*>(q + h * p.q_s1), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] += (double)(upper ? (f[i] < 0.f ? 0.f : f[i]) : (f[i] > 0.f ? 0.f : f[i]));
+    }
+    uint64_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride + i0;
+    for (int j = 0; j < steps; ++j) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      double s[kStep];
+#pragma unroll
+      for (int u = 0; u < kStep; ++u) {
+        const uint4 v = *reinterpret_cast<const uint4*>(ring + ((j % kRing * kStep + u) * kThreads + tid) * 16);
         float f[8];
-        to_f32x8(T{}, v[u], f);
+        to_f32x8(T{}, v, f);
         s[u] = 0.0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[u] = fma((double)f[i], w[i], s[u]);
       }
-      // sums over the LP lanes of a page: three steps that also halve the pages a lane holds
+      if (j + 2 < steps) issue(j + 2);   // into the slots of step j - 1
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      // sums over the LP lanes of a page: first steps that also halve the pages a lane holds
+      int at = j * kPer + sub * kStep, o = LP / 2;
 #pragma unroll
-      for (int h = 4, o = LP / 2; h >= 1; h >>= 1, o >>= 1)
+      for (int h = kStep / 2; h >= 1; h >>= 1, o >>= 1) {
 #pragma unroll
         for (int i = 0; i < h; ++i) {
           const double give = lane & o ? s[i] : s[i + h], keep = lane & o ? s[i + h] : s[i];
           s[i] = keep + __shfl_xor_sync(~0u, give, o);
         }
-#pragma unroll
-      for (int o = LP / 16; o; o >>= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
-      const int at = i0 + sub * 8 + (lane & (LP / 2) ? 4 : 0) + (lane & (LP / 4) ? 2 : 0) + (lane & (LP / 8) ? 1 : 0);
-      if ((lane & (LP / 8 - 1)) == 0 && at < cnt) {
-        const uint64_t key = order_key(s[0]);
-        keys[at] = key;
-        k_lo = min(k_lo, key);
-        k_hi = max(k_hi, key);
+        at += lane & o ? h : 0;
       }
+      const int last = o;                            // lanes below: copies of the same page
+#pragma unroll
+      for (; o; o >>= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
+      if ((lane & (2 * last - 1)) == 0 && i0 + at < i1) keys[at] = order_key(s[0]);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    g += here;
+    run = 0;
+    if (g < g1 && ++hk == p.num_kv_heads) {
+      hk = 0;
+      do N = ++b < p.n ? competing(p, pages_of(p, b)) : 0;
+      while (N == 0 && b < p.n);
+      if (b >= p.n) break;   // not reached: g < g1 <= total
+      runs = (N + kRun - 1) / kRun;
+    }
+  }
+}
+
+constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
+
+__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectPagesParams p) {
+  __shared__ uint32_t hist[256];
+  __shared__ uint64_t warp_lo[kPickWarps], warp_hi[kPickWarps];
+  __shared__ uint32_t scan[8], found[3];             // bin, still needed in it, its count
+  __shared__ int n_gt[kPickWarps], n_eq[kPickWarps];
+  const int unit = blockIdx.x;
+  const int hk = unit % p.num_kv_heads, b = unit / p.num_kv_heads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int P = pages_of(p, b), N = competing(p, P);
+  // the attention over the lists may take the place of CTAs that are done; it waits for all
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int32_t* out = p.pages + b * p.pg_s0 + hk * p.pg_s1;
+  if (P <= p.top) {   // every page, then -1
+    for (int i = tid; i < p.top; i += kPickThreads) out[i] = i < P ? i : -1;
+  } else {
+    for (int i = tid; i < p.sinks; i += kPickThreads) out[i] = i;
+    for (int i = tid; i < p.recent; i += kPickThreads) out[p.top - p.recent + i] = P - p.recent + i;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the scores are written
+  if (N == 0) return;
+  const uint64_t* keys = p.keys + (int64_t)unit * p.key_stride;
+  constexpr int kAhead = 4;                          // keys in flight per thread
+
+  uint64_t k_lo = ~0ull, k_hi = 0;
+  for (int i = tid; i < N; i += kAhead * kPickThreads) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint64_t k = keys[min(i + u * kPickThreads, N - 1)];
+      k_lo = min(k_lo, k);
+      k_hi = max(k_hi, k);
     }
   }
 #pragma unroll
@@ -224,56 +290,51 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectPagesParam
     warp_lo[warp] = k_lo;
     warp_hi[warp] = k_hi;
   }
-  hist[0][tid] = 0;
+  if (tid < 256) hist[tid] = 0;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) {
-      k_lo = min(k_lo, warp_lo[w]);
-      k_hi = max(k_hi, warp_hi[w]);
-    }
-    range[0] = k_lo;
-    range[1] = k_hi;
-  }
-  cluster.sync();
-  k_lo = ~0ull;
-  k_hi = 0;
-  for (int r = 0; r < C; ++r) {
-    const uint64_t* o = cluster.map_shared_rank(range, r);
-    k_lo = min(k_lo, o[0]);
-    k_hi = max(k_hi, o[1]);
+#pragma unroll
+  for (int w = 0; w < kPickWarps; ++w) {
+    k_lo = min(k_lo, warp_lo[w]);
+    k_hi = max(k_hi, warp_hi[w]);
   }
 
   // ---- the border: key >> shift == border for the last selected ones, `rest` of them ----
   const int top_bit = k_lo == k_hi ? -1 : 63 - __clzll((long long)(k_lo ^ k_hi));
   int shift = top_bit + 1;                           // bits above are the same in all keys
   uint64_t border = shift >= 64 ? 0 : k_lo >> shift;
-  int rest = need;
-  for (int pass = 0; shift > 0; ++pass) {
+  int rest = p.top - p.sinks - p.recent;             // < N
+  while (shift > 0) {
     const int bits = min(8, shift), ns = shift - bits;
-    uint32_t* h = hist[pass & 1];
-    for (int i = tid; i < cnt; i += kThreads) {
-      const uint64_t k = keys[i];
-      if (shift >= 64 || (k >> shift) == border) atomicAdd(&h[(uint32_t)(k >> ns) & ((1u << bits) - 1)], 1u);
-    }
-    cluster.sync();
-    // bins from the highest down: thread t has bin 255 - t
-    const int bin = 255 - tid;
-    uint32_t mine = 0;
-    for (int r = 0; r < C; ++r) mine += cluster.map_shared_rank(h, r)[bin];
-    hist[(pass + 1) & 1][tid] = 0;                   // its readers passed the barrier above
-    uint32_t incl = mine;
+    for (int i = tid; i < N; i += kAhead * kPickThreads) {
+      uint64_t k[kAhead];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(~0u, incl, o);
-      if (lane >= o) incl += v;
+      for (int u = 0; u < kAhead; ++u) k[u] = keys[min(i + u * kPickThreads, N - 1)];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u * kPickThreads < N && (shift >= 64 || (k[u] >> shift) == border))
+          atomicAdd(&hist[(uint32_t)(k[u] >> ns) & ((1u << bits) - 1)], 1u);
     }
-    if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) incl += scan[w];
-    if (incl >= (uint32_t)rest && incl - mine < (uint32_t)rest) {
-      found[0] = (uint32_t)bin;
-      found[1] = (uint32_t)rest - (incl - mine);
-      found[2] = mine;
+    // bins from the highest down: thread t < 256 has bin 255 - t
+    uint32_t mine = 0, incl = 0;
+    if (warp < 8) {
+      mine = incl = hist[255 - tid];
+      hist[255 - tid] = 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(~0u, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) scan[warp] = incl;
+    }
+    __syncthreads();
+    if (warp < 8) {
+      for (int w = 0; w < warp; ++w) incl += scan[w];
+      if (incl >= (uint32_t)rest && incl - mine < (uint32_t)rest) {
+        found[0] = 255 - (uint32_t)tid;
+        found[1] = (uint32_t)rest - (incl - mine);
+        found[2] = mine;
+      }
     }
     __syncthreads();
     border = (border << bits) | found[0];
@@ -282,43 +343,22 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectPagesParam
     if (found[2] == found[1]) break;                 // the whole bin is selected
   }
 
-  // ---- the selected pages in ascending order ----
-  const int per = ((cnt + kWarps - 1) / kWarps + 31) & ~31;
-  const int w0 = min(warp * per, cnt), w1 = min(w0 + per, cnt);
+  // ---- the selected pages in ascending order: a warp per consecutive part ----
+  const int per = ((N + kPickWarps - 1) / kPickWarps + 31) & ~31;
+  const int w0 = min(warp * per, N), w1 = min(w0 + per, N);
   int gt = 0, eq = 0;
   for (int i0 = w0; i0 < w1; i0 += 32) {
-    const uint64_t k = i0 + lane < w1 ? keys[i0 + lane] >> shift : 0;
-    gt += __popc(__ballot_sync(~0u, i0 + lane < w1 && k > border));
-    eq += __popc(__ballot_sync(~0u, i0 + lane < w1 && k == border));
+    const bool in = i0 + lane < w1;
+    const uint64_t k = in ? keys[i0 + lane] >> shift : 0;
+    gt += __popc(__ballot_sync(~0u, in && k > border));
+    eq += __popc(__ballot_sync(~0u, in && k == border));
   }
   if (lane == 0) {
     n_gt[warp] = gt;
     n_eq[warp] = eq;
   }
   __syncthreads();
-  if (tid == 0) {
-    int a = 0, c = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      a += n_gt[w];
-      c += n_eq[w];
-    }
-    cta_counts[0] = a;
-    cta_counts[1] = c;
-  }
-  cluster.sync();
-  if (tid == 0) {
-    int a = 0, c = 0;
-    for (int r = 0; r < rank; ++r) {
-      const int* o = cluster.map_shared_rank(cta_counts, r);
-      a += o[0];
-      c += o[1];
-    }
-    before[0] = a;
-    before[1] = c;
-  }
-  __syncthreads();
-  gt = before[0];
-  eq = before[1];
+  gt = eq = 0;
   for (int w = 0; w < warp; ++w) {
     gt += n_gt[w];
     eq += n_eq[w];
@@ -328,43 +368,36 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectPagesParam
     const uint64_t k = in ? keys[i0 + lane] >> shift : 0;
     const uint32_t mg = __ballot_sync(~0u, in && k > border), me = __ballot_sync(~0u, in && k == border);
     const uint32_t below = (1u << lane) - 1u;
-    const int g = gt + __popc(mg & below), e = eq + __popc(me & below);
-    if (in && (k > border || (k == border && e < rest))) out[p.sinks + g + min(e, rest)] = p.sinks + c0 + i0 + lane;
+    const int gb = gt + __popc(mg & below), eb = eq + __popc(me & below);
+    if (in && (k > border || (k == border && eb < rest))) out[p.sinks + gb + min(eb, rest)] = p.sinks + i0 + lane;
     gt += __popc(mg);
     eq += __popc(me);
   }
-  cluster.sync();   // no CTA leaves while another reads its counts
 }
 
 template <typename T, int D>
 int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
-  const int64_t most = ((int64_t)p.max_len + p.block_size - 1) / p.block_size;
   const int64_t units = (int64_t)p.n * p.num_kv_heads;
-  // a cluster per unit: more CTAs while the units alone leave SMs idle and a CTA keeps
-  // at least 64 pages, and as many as the scores need in shared memory
-  int C = 1;
-  while (C < kMaxCluster && units * C < 2 * num_sms && most / (2 * C) >= 64) C *= 2;
-  while (C < kMaxCluster && (size_t)((most + C - 1) / C + 1) * 8 > kKeyBytes) C *= 2;
-  const size_t smem = (size_t)((most + C - 1) / C + 1) * 8;
-  if (smem > kKeyBytes || units * C > 0x7fffffff) return STARKV_EINVAL;
-  p.keys = (int)((most + C - 1) / C + 1);
-  const void* fn = (const void*)select_kernel<T, D>;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kKeyBytes) != cudaSuccess)
-    return STARKV_ECUDA;
+  if (units * ((p.key_stride + kRun - 1) / kRun) > 0x7fffffff) return STARKV_EINVAL;   // 32-bit run numbers
+  const void* fn = (const void*)score_kernel<T, D>;
+  if (const int st = allow_smem(fn, kRingBytes)) return st;
+  void* args[] = {&p};
+  if (p.key_stride > p.top) {   // else no sequence has pages to choose from
+    const int64_t runs = units * ((p.key_stride + kRun - 1) / kRun);
+    const int64_t grid = std::min<int64_t>(3 * num_sms, runs);
+    if (cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), args, kRingBytes, stream) != cudaSuccess)
+      return STARKV_ECUDA;
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(units * C));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)units);
+  cfg.blockDim = dim3(kPickThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  void* args[] = {&p};
-  return cudaLaunchKernelExC(&cfg, fn, args) == cudaSuccess ? STARKV_OK : STARKV_ECUDA;
+  cfg.numAttrs = p.key_stride > p.top;   // behind score_kernel alone may the launch come early
+  return cudaLaunchKernelExC(&cfg, (const void*)pick_kernel, args) == cudaSuccess ? STARKV_OK : STARKV_ECUDA;
 }
 
 template <typename T, int D>

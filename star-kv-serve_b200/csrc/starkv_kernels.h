@@ -147,6 +147,8 @@ struct PagedAttnParams {
   int n, num_heads, group;                           // group: query heads per KV head
   int head_groups, units;                            // ceil(group / 16); KV heads * head_groups
   int max_unit_tokens;                               // host bound on the tokens of a unit
+  int after_select;                                  // 1: the page lists come from pick_kernel, launched just before
+  int item_shift;                                    // set by the launch: log2 of a work item's tokens
   float scale;
   void* out; int64_t o_s0, o_s1;
   float* m_out; float* l_out;                        // set: the partial form (out f32, not divided)
@@ -172,7 +174,7 @@ struct SelectPagesParams {
   int max_blocks, num_blocks, block_size;
   const int32_t* seq_lens;
   int max_len, n, num_kv_heads, group, top, sinks, recent;
-  int keys;                                          // score slots of one CTA (shared memory)
+  uint64_t* keys; int64_t key_stride;                // scratch [n, KV heads, pages of the longest sequence]
   int32_t* pages; int64_t pg_s0, pg_s1;              // [n, KV heads, top]
   int32_t* status;
 };
@@ -219,6 +221,9 @@ int kv_down_ctl_offset(int n_tile, int stages);
 int kv_down_split();
 int launch_kv_down_write(const CUtensorMap& tm_w, const CUtensorMap& tm_x, const DownWriteParams& p,
                          cudaStream_t stream);
+// cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel on the current device, set by
+// its first launch there.
+int allow_smem(const void* fn, int bytes);
 size_t paged_attn_workspace_bytes(int rows, int head_dim, int max_tokens);
 int launch_paged_attn(const PagedAttnParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
 int launch_page_bounds(const PageBoundsParams& p, int dtype, int head_dim, cudaStream_t stream);

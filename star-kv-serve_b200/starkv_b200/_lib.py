@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -121,6 +122,21 @@ class NormRopeArgs(C.Structure):
     ]
 
 
+def _packed(cls):
+    """``pack(*values)`` -> the bytes of an argument struct, array members flattened. The
+    operators of the full-rank paged cache are short enough on the GPU for the filling of
+    a ctypes structure (about 15 us) to show; one struct.pack takes 2."""
+    fmt = ""
+    for _, t in cls._fields_:
+        n, t = (t._length_, t._type_) if issubclass(t, C.Array) else (1, t)
+        fmt += f"{n}{ {p: 'Q', i64: 'q', i32: 'i', f32: 'f'}[t] }"
+    pad = C.sizeof(cls) - struct.calcsize("@" + fmt)
+    return struct.Struct(f"@{fmt}{pad}x").pack
+
+
+pack_paged_attn, pack_page_bounds = _packed(PagedAttnArgs), _packed(PageBoundsArgs)
+pack_select_pages, pack_norm_rope = _packed(SelectPagesArgs), _packed(NormRopeArgs)
+
 EXPORTS = {
     "starkv_decode_workspace_bytes": (C.c_size_t, [i32, i32, i32, i32, i32, i32]),
     "starkv_paged_decode_bf16": (C.c_int, [C.POINTER(DecodeArgs), p, C.c_size_t, p]),
@@ -138,10 +154,12 @@ EXPORTS = {
     "starkv_prefill_attention": (C.c_int, [p, C.POINTER(i64), p, C.POINTER(i64), p, C.POINTER(i64), i32, i32, i32, i32,
                                            i32, p, i32, i32, f32, p, C.POINTER(i64), p, p]),
     "starkv_paged_attention_workspace_bytes": (C.c_size_t, [i32, i32, i32, i32]),
-    "starkv_paged_attention": (C.c_int, [C.POINTER(PagedAttnArgs), p, C.c_size_t, p]),
-    "starkv_page_bounds": (C.c_int, [C.POINTER(PageBoundsArgs), p]),
-    "starkv_select_pages": (C.c_int, [C.POINTER(SelectPagesArgs), p]),
-    "starkv_norm_rope": (C.c_int, [C.POINTER(NormRopeArgs), p]),
+    "starkv_paged_attention": (C.c_int, [C.c_char_p, p, C.c_size_t, p]),
+    "starkv_page_bounds": (C.c_int, [C.c_char_p, p]),
+    "starkv_select_pages_workspace_bytes": (C.c_size_t, [i32, i32, i32, i32, i32]),
+    "starkv_select_pages": (C.c_int, [C.c_char_p, p, C.c_size_t, p]),
+    "starkv_sparse_paged_attention": (C.c_int, [C.c_char_p, p, i64, i64, i32, i32, p, C.c_size_t, p]),
+    "starkv_norm_rope": (C.c_int, [C.c_char_p, p]),
     "starkv_cache_write_bf16": (C.c_int, [C.POINTER(CacheWriteArgs), p]),
     "starkv_read_status": (C.c_int, [p, C.POINTER(i32), i32, p]),
     "starkv_status_offset": (C.c_size_t, []),
@@ -199,33 +217,35 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def addr(t: torch.Tensor | None) -> int:
+    """Address for the pack_* functions, which take 0 for a null pointer."""
+    return 0 if t is None else t.data_ptr()
+
+
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def same_device(what: str, **tensors) -> torch.device:
-    """The one CUDA device of the given tensors (None: left out); ValueError otherwise."""
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{what}: {name} must be a CUDA tensor")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{what}: {name} is on {t.device}, not on {dev}")
-    return dev
+def same_device(what: str, *tensors) -> int:
+    """Index of the one CUDA device of the given tensors (None: left out); ValueError otherwise."""
+    idx = None
+    for t in tensors:
+        if t is not None and t.get_device() != idx:
+            if idx is not None or t.get_device() < 0:
+                raise ValueError(f"{what}: all tensors must be on one CUDA device")
+            idx = t.get_device()
+    return idx
 
 
-def launch(what: str, device: torch.device, fn, *args) -> None:
-    """``fn(*args, stream)`` on the current stream of `device`, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        st = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def launch(what: str, idx: int, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of device `idx`, whichever device is current."""
+    if idx == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
-        with torch.cuda.device(device):
-            st = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    check(st, what)
+        with torch.cuda.device(idx):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if st:
+        check(st, what)
 
 
 def i64s(values):

@@ -21,7 +21,6 @@ import torch
 from .. import _lib, context_parallel
 
 HEAD_DIMS = (64, 128)
-_i2, _i3 = _lib.i64 * 2, _lib.i64 * 3
 
 
 def empty_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int = 128, dtype=torch.bfloat16,
@@ -97,7 +96,14 @@ def paged_attention_decode(
     ``ws``: scratch of this call alone (``workspace_bytes``); by default it is
     allocated on the current stream, so that calls that overlap, or captured graphs
     that are replayed at once, do not share it."""
-    what = "paged_attention_decode"
+    return _attend("paged_attention_decode", query, k_cache, v_cache, block_table, seq_lens, max_seq_len, scale, pages,
+                   out, return_partial, partial, ws, status)
+
+
+def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, scale, pages, out, return_partial, partial,
+            ws, status, select=None):
+    """The checks and the call of the attention; ``select`` = (bounds, sinks, recent): the
+    pages are selected first, in the same call of the library."""
     _check_cache(what, k_cache, "k_cache", query.dtype)
     _check_cache(what, v_cache, "v_cache", query.dtype)
     if k_cache.shape != v_cache.shape:
@@ -126,21 +132,27 @@ def paged_attention_decode(
         out = torch.empty((n, hq, d), dtype=query.dtype, device=query.device)
     elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must be [{n}, {hq}, {d}] in the cache's dtype, last dimension contiguous")
-    dev = _lib.same_device(what, query=query, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
-                           seq_lens=seq_lens, pages=pages, out=out, ws=ws, status=status)
+    bounds = None if select is None else select[0]
+    idx = _lib.same_device(what, query, k_cache, v_cache, block_table, seq_lens, pages, out, ws, status, bounds)
     if n == 0:
         return (out, m, l) if return_partial else out
-    lib = _lib.lib()
     if ws is None:
-        ws = torch.empty(workspace_bytes(hq, hkv, d, top * bs if top else int(max_seq_len)), dtype=torch.uint8,
-                         device=dev)
-    a = _lib.PagedAttnArgs(
-        query.data_ptr(), _i2(*query.stride()[:2]), k_cache.data_ptr(), _i3(*k_cache.stride()[:3]),
-        v_cache.data_ptr(), _i3(*v_cache.stride()[:3]), block_table.data_ptr(), _i2(*block_table.stride()),
-        seq_lens.data_ptr(), None if pages is None else pages.data_ptr(), _i2(*pg), out.data_ptr(),
-        _i2(*out.stride()[:2]), _lib.ptr(m), _lib.ptr(l), _lib.ptr(status), _lib.dtype_code(query), n, hq, hkv, d, nb, bs,
+        need = workspace_bytes(hq, hkv, d, top * bs if top else int(max_seq_len))
+        if select is not None:
+            need += select_workspace_bytes(n, hkv, int(max_seq_len), bs, top)
+        ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    P = _lib.addr
+    a = _lib.pack_paged_attn(
+        query.data_ptr(), *query.stride()[:2], k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(),
+        *v_cache.stride()[:3], block_table.data_ptr(), *block_table.stride(), seq_lens.data_ptr(), P(pages), *pg,
+        out.data_ptr(), *out.stride()[:2], P(m), P(l), P(status), _lib.dtype_code(query), n, hq, hkv, d, nb, bs,
         block_table.shape[1], int(max_seq_len), top, float(scale))
-    _lib.launch(what, dev, lib.starkv_paged_attention, a, ws.data_ptr(), ws.numel() * ws.element_size())
+    size = 0 if ws is None else ws.nbytes
+    if select is None:
+        _lib.launch(what, idx, _lib.lib().starkv_paged_attention, a, P(ws), size)
+    else:
+        _lib.launch(what, idx, _lib.lib().starkv_sparse_paged_attention, a, bounds.data_ptr(), *bounds.stride()[:2],
+                    select[1], select[2], P(ws), size)
     return (out, m, l) if return_partial else out
 
 
@@ -148,6 +160,13 @@ def workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int, max_tokens
     """Scratch of one ``paged_attention_decode`` over at most ``max_tokens`` tokens per sequence."""
     return int(_lib.lib().starkv_paged_attention_workspace_bytes(num_heads, num_kv_heads, head_dim,
                                                                   min(int(max_tokens), 1 << 30)))
+
+
+def select_workspace_bytes(n: int, num_kv_heads: int, max_seq_len: int, block_size: int, top: int) -> int:
+    """Scratch of one ``select_pages``; ``sparse_paged_decode`` takes this and ``workspace_bytes``
+    of top * block_size tokens."""
+    return int(_lib.lib().starkv_select_pages_workspace_bytes(n, num_kv_heads, min(int(max_seq_len), 1 << 30),
+                                                              block_size, top))
 
 
 def update_page_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -170,25 +189,15 @@ def update_page_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table:
         if tuple(new_lens.shape) != (n,):
             raise ValueError(f"{what}: new_lens must be [{n}]")
         new_lens = _i32(new_lens).contiguous()
-    dev = _lib.same_device(what, k_cache=k_cache, bounds=bounds, block_table=block_table, seq_lens=seq_lens,
-                           new_lens=new_lens, status=status)
-    a = _lib.PageBoundsArgs(
-        k_cache.data_ptr(), _i3(*k_cache.stride()[:3]), bounds.data_ptr(), _i2(*bounds.stride()[:2]),
-        block_table.data_ptr(), _i2(*block_table.stride()), seq_lens.data_ptr(), _lib.ptr(new_lens), _lib.ptr(status),
-        _lib.dtype_code(k_cache), n, hkv, d, nb, bs, block_table.shape[1], int(max_seq_len), int(max_new))
-    _lib.launch(what, dev, _lib.lib().starkv_page_bounds, a)
+    idx = _lib.same_device(what, k_cache, bounds, block_table, seq_lens, new_lens, status)
+    a = _lib.pack_page_bounds(
+        k_cache.data_ptr(), *k_cache.stride()[:3], bounds.data_ptr(), *bounds.stride()[:2], block_table.data_ptr(),
+        *block_table.stride(), seq_lens.data_ptr(), _lib.addr(new_lens), _lib.addr(status), _lib.dtype_code(k_cache),
+        n, hkv, d, nb, bs, block_table.shape[1], int(max_seq_len), int(max_new))
+    _lib.launch(what, idx, _lib.lib().starkv_page_bounds, a)
 
 
-def select_pages(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
-                 max_seq_len: int, block_size: int, top: int, *, sinks: int = 1, recent: int = 1,
-                 out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
-    """The ``top`` pages per sequence and KV head with the largest
-    ``sum_{g, d} max(q[g, d] lo[d], q[g, d] hi[d])`` over the head's query heads g:
-    int32 [n, H_kv, top], ascending, -1 behind them where a sequence has fewer pages.
-    The first ``sinks`` and the last ``recent`` pages are always among them (the last
-    page is usually not full, and its bounds need not be up to date while recent >= 1).
-    Scores in 64 bits; ties go to the lowest page; a NaN score ranks above all others."""
-    what = "select_pages"
+def _check_bounds(what: str, query, bounds, top, sinks, recent):
     if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.shape[3] not in HEAD_DIMS:
         raise ValueError(f"{what}: bounds must be [num_blocks, H_kv, 2, 64 or 128]")
     nb, hkv, _, d = bounds.shape
@@ -196,25 +205,42 @@ def select_pages(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.T
         raise ValueError(f"{what}: query and bounds must be bf16 or f16, both the same")
     if bounds.stride(-1) != 1 or bounds.stride(-2) != d:
         raise ValueError(f"{what}: the (lo, hi) rows of bounds must be contiguous")
-    _check_query(what, query, hkv, d)
-    n, hq, _ = query.shape
     if top < 1 or sinks < 0 or recent < 0 or sinks + recent > top:
         raise ValueError(f"{what}: need top >= 1 and sinks + recent <= top")
+    return nb, hkv, d
+
+
+def select_pages(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                 max_seq_len: int, block_size: int, top: int, *, sinks: int = 1, recent: int = 1,
+                 out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None) -> torch.Tensor:
+    """The ``top`` pages per sequence and KV head with the largest
+    ``sum_{g, d} max(q[g, d] lo[d], q[g, d] hi[d])`` over the head's query heads g:
+    int32 [n, H_kv, top], ascending, -1 behind them where a sequence has fewer pages.
+    The first ``sinks`` and the last ``recent`` pages are always among them (the last
+    page is usually not full, and its bounds need not be up to date while recent >= 1).
+    Scores in 64 bits; ties go to the lowest page; a NaN score ranks above all others."""
+    what = "select_pages"
+    nb, hkv, d = _check_bounds(what, query, bounds, top, sinks, recent)
+    _check_query(what, query, hkv, d)
+    n, hq, _ = query.shape
     block_table, seq_lens = _check_table(what, n, block_table, seq_lens)
     if out is None:
         out = torch.empty((n, hkv, top), dtype=torch.int32, device=query.device)
     elif tuple(out.shape) != (n, hkv, top) or out.dtype != torch.int32 or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must be int32 [{n}, {hkv}, {top}], last dimension contiguous")
-    dev = _lib.same_device(what, query=query, bounds=bounds, block_table=block_table, seq_lens=seq_lens, out=out,
-                           status=status)
+    idx = _lib.same_device(what, query, bounds, block_table, seq_lens, out, ws, status)
     if n == 0:
         return out
-    a = _lib.SelectPagesArgs(
-        query.data_ptr(), _i2(*query.stride()[:2]), bounds.data_ptr(), _i2(*bounds.stride()[:2]),
-        block_table.data_ptr(), _i2(*block_table.stride()), seq_lens.data_ptr(), out.data_ptr(), _i2(*out.stride()[:2]),
-        _lib.ptr(status), _lib.dtype_code(query), n, hq, hkv, d, nb, int(block_size), block_table.shape[1],
-        int(max_seq_len), int(top), int(sinks), int(recent))
-    _lib.launch(what, dev, _lib.lib().starkv_select_pages, a)
+    if ws is None:
+        need = select_workspace_bytes(n, hkv, max_seq_len, block_size, top)
+        ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    a = _lib.pack_select_pages(
+        query.data_ptr(), *query.stride()[:2], bounds.data_ptr(), *bounds.stride()[:2], block_table.data_ptr(),
+        *block_table.stride(), seq_lens.data_ptr(), out.data_ptr(), *out.stride()[:2], _lib.addr(status),
+        _lib.dtype_code(query), n, hq, hkv, d, nb, int(block_size), block_table.shape[1], int(max_seq_len), int(top),
+        int(sinks), int(recent))
+    _lib.launch(what, idx, _lib.lib().starkv_select_pages, a, _lib.addr(ws), 0 if ws is None else ws.nbytes)
     return out
 
 
@@ -225,10 +251,11 @@ def sparse_paged_decode(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """``select_pages``, then ``paged_attention_decode`` over those pages: (out, pages).
     ``bounds`` as ``update_page_bounds`` keeps them. With top >= the pages of a sequence
     this is the attention over all of it."""
-    if bounds.shape[:2] != (k_cache.shape[0], k_cache.shape[2]):
-        raise ValueError("sparse_paged_decode: bounds and cache must have the same blocks and heads")
-    pages = select_pages(query, bounds, block_table, seq_lens, max_seq_len, k_cache.shape[1], top, sinks=sinks,
-                         recent=recent, status=status)
-    out = paged_attention_decode(query, k_cache, v_cache, block_table, seq_lens, max_seq_len, scale, pages=pages,
-                                 out=out, ws=ws, status=status)
+    what = "sparse_paged_decode"
+    nb, hkv, d = _check_bounds(what, query, bounds, top, sinks, recent)
+    if (nb, hkv, d) != (k_cache.shape[0], *k_cache.shape[2:]):
+        raise ValueError(f"{what}: bounds and cache must have the same blocks, heads and head_dim")
+    pages = torch.empty((query.shape[0], hkv, top), dtype=torch.int32, device=query.device)
+    out = _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, scale, pages, out, False, None, ws,
+                  status, select=(bounds, int(sinks), int(recent)))
     return out, pages

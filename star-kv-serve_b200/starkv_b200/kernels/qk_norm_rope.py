@@ -15,8 +15,7 @@ import torch
 from .. import _lib
 from .paged_attention import HEAD_DIMS, _check_cache
 
-_i2, _i3 = _lib.i64 * 2, _lib.i64 * 3
-_Z2, _Z3 = _i2(0, 0), _i3(0, 0, 0)
+_Z2, _Z3 = (0, 0), (0, 0, 0)
 
 
 def _rows(what: str, name: str, t: torch.Tensor, n: int, heads: int, d: int, dtype) -> None:
@@ -69,22 +68,20 @@ def _run(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping
     if k_out is not None:
         _rows(what, "k_out", k_out, n, hkv, d, q.dtype)
     positions = positions.contiguous()
-    dev = _lib.same_device(what, q=q, k=k, v=v, positions=positions, cos_sin_cache=cos_sin_cache, k_cache=k_cache,
-                           v_cache=v_cache, slot_mapping=slot_mapping, q_weight=q_weight, k_weight=k_weight,
-                           q_out=q_out, k_out=k_out, status=status)
+    idx = _lib.same_device(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping, q_weight, k_weight,
+                           q_out, k_out, status)
     if n == 0:
         return q_out
-    P = _lib.ptr
-    a = _lib.NormRopeArgs(
-        q.data_ptr(), _i2(*q.stride()[:2]), P(k), _Z2 if k is None else _i2(*k.stride()[:2]),
-        P(v), _Z2 if v is None else _i2(*v.stride()[:2]), q_out.data_ptr(), _i2(*q_out.stride()[:2]),
-        P(k_out), _Z2 if k_out is None else _i2(*k_out.stride()[:2]), P(q_weight), P(k_weight),
-        positions.data_ptr(), cos_sin_cache.data_ptr(), cos_sin_cache.stride(0),
-        P(k_cache), _Z3 if k_cache is None else _i3(*k_cache.stride()[:3]),
-        P(v_cache), _Z3 if v_cache is None else _i3(*v_cache.stride()[:3]), P(slot_mapping), P(status),
-        _lib.dtype_code(q), w_dtype, _lib.dtype_code(positions), _lib.dtype_code(cos_sin_cache), slot_dtype,
-        n, hq, hkv, d, cos_sin_cache.shape[1], cos_sin_cache.shape[0], nb, bs, float(eps))
-    _lib.launch(what, dev, _lib.lib().starkv_norm_rope, a)
+    P = _lib.addr
+    a = _lib.pack_norm_rope(
+        q.data_ptr(), *q.stride()[:2], P(k), *(_Z2 if k is None else k.stride()[:2]),
+        P(v), *(_Z2 if v is None else v.stride()[:2]), q_out.data_ptr(), *q_out.stride()[:2],
+        P(k_out), *(_Z2 if k_out is None else k_out.stride()[:2]), P(q_weight), P(k_weight), positions.data_ptr(),
+        cos_sin_cache.data_ptr(), cos_sin_cache.stride(0), P(k_cache), *(_Z3 if k_cache is None else k_cache.stride()[:3]),
+        P(v_cache), *(_Z3 if v_cache is None else v_cache.stride()[:3]), P(slot_mapping), P(status), _lib.dtype_code(q),
+        w_dtype, _lib.dtype_code(positions), _lib.dtype_code(cos_sin_cache), slot_dtype, n, hq, hkv, d,
+        cos_sin_cache.shape[1], cos_sin_cache.shape[0], nb, bs, float(eps))
+    _lib.launch(what, idx, _lib.lib().starkv_norm_rope, a)
     return q_out
 
 
