@@ -226,20 +226,21 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def same_device(what: str, *tensors) -> int:
-    """Index of the one CUDA device of the given tensors (None: left out); ValueError otherwise."""
-    idx = None
-    for t in tensors:
+def same_device(what: str, first: torch.Tensor, *rest) -> int:
+    """Index of the CUDA device that all tensors (None: left out) are on; ValueError otherwise."""
+    idx = first.get_device()
+    for t in rest:
         if t is not None and t.get_device() != idx:
-            if idx is not None or t.get_device() < 0:
-                raise ValueError(f"{what}: all tensors must be on one CUDA device")
-            idx = t.get_device()
+            idx = -1
+            break
+    if idx < 0:
+        raise ValueError(f"{what}: all tensors must be on one CUDA device")
     return idx
 
 
 def launch(what: str, idx: int, fn, *args) -> None:
     """``fn(*args, stream)`` on the current stream of device `idx`, whichever device is current."""
-    if idx == torch.cuda.current_device():
+    if idx == torch._C._cuda_getDevice():
         st = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):

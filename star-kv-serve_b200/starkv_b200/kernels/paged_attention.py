@@ -37,31 +37,35 @@ def empty_bounds(k_cache: torch.Tensor) -> torch.Tensor:
     return torch.zeros(nb, hkv, 2, d, dtype=k_cache.dtype, device=k_cache.device)
 
 
-def _i32(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dtype == torch.int32 else t.to(torch.int32)
+_CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}   # the cache's element types
 
 
-def _check_table(what: str, n: int, block_table: torch.Tensor, seq_lens: torch.Tensor):
-    if block_table.dim() != 2 or block_table.shape[0] != n or tuple(seq_lens.shape) != (n,):
+def _tables(what: str, n: int, block_table: torch.Tensor, seq_lens: torch.Tensor):
+    """(block_table, seq_lens) as int32, the lengths contiguous."""
+    if block_table.dim() != 2 or block_table.shape[0] != n or seq_lens.shape != (n,):
         raise ValueError(f"{what}: block_table must be [{n}, max_blocks] and seq_lens [{n}]")
-    seq_lens = _i32(seq_lens)
-    return _i32(block_table), seq_lens if seq_lens.is_contiguous() else seq_lens.contiguous()
+    if block_table.dtype is not torch.int32:
+        block_table = block_table.to(torch.int32)
+    if seq_lens.dtype is not torch.int32 or not seq_lens.is_contiguous():
+        seq_lens = seq_lens.to(torch.int32).contiguous()
+    return block_table, seq_lens
 
 
-def _check_cache(what: str, cache: torch.Tensor, name: str, dtype: torch.dtype) -> None:
-    if cache.dim() != 4 or cache.shape[-1] not in HEAD_DIMS:
-        raise ValueError(f"{what}: {name} must be [num_blocks, block_size, H_kv, 64 or 128]")
-    if cache.dtype != dtype or dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"{what}: query and cache must be bf16 or f16, all the same")
-    if cache.stride(-1) != 1:
-        raise ValueError(f"{what}: {name} needs a contiguous last dimension")
+def _cache_sizes(what: str, name: str, cache: torch.Tensor, dtype: torch.dtype):
+    """The sizes of a cache tensor, checked against the call's element type."""
+    sizes = cache.shape
+    if len(sizes) != 4 or sizes[3] not in HEAD_DIMS or cache.stride(3) != 1:
+        raise ValueError(f"{what}: {name} must be [num_blocks, block_size, H_kv, 64 or 128], last dimension contiguous")
+    if cache.dtype is not dtype or dtype not in _CODES:
+        raise ValueError(f"{what}: all tensors must be bf16 or f16, the same as the cache")
+    return sizes
 
 
-def _check_query(what: str, query: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
-    if query.dim() != 3 or query.shape[2] != head_dim or query.shape[1] == 0 or query.shape[1] % num_kv_heads:
-        raise ValueError(f"{what}: query must be [n, multiple of {num_kv_heads}, {head_dim}]")
-    if query.stride(-1) != 1:
-        raise ValueError(f"{what}: query needs a contiguous last dimension")
+def _query_sizes(what: str, query: torch.Tensor, num_kv_heads: int, head_dim: int):
+    sizes = query.shape
+    if len(sizes) != 3 or sizes[2] != head_dim or sizes[1] == 0 or sizes[1] % num_kv_heads or query.stride(2) != 1:
+        raise ValueError(f"{what}: query must be [n, multiple of {num_kv_heads}, {head_dim}], last dimension contiguous")
+    return sizes
 
 
 def paged_attention_decode(
@@ -104,17 +108,14 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
             ws, status, select=None):
     """The checks and the call of the attention; ``select`` = (bounds, sinks, recent): the
     pages are selected first, in the same call of the library."""
-    _check_cache(what, k_cache, "k_cache", query.dtype)
-    _check_cache(what, v_cache, "v_cache", query.dtype)
-    if k_cache.shape != v_cache.shape:
+    nb, bs, hkv, d = _cache_sizes(what, "k_cache", k_cache, query.dtype)
+    if _cache_sizes(what, "v_cache", v_cache, query.dtype) != k_cache.shape:
         raise ValueError(f"{what}: k_cache and v_cache must have the same shape")
-    nb, bs, hkv, d = k_cache.shape
-    _check_query(what, query, hkv, d)
-    n, hq, _ = query.shape
-    block_table, seq_lens = _check_table(what, n, block_table, seq_lens)
+    n, hq, _ = _query_sizes(what, query, hkv, d)
+    block_table, seq_lens = _tables(what, n, block_table, seq_lens)
     top, pg = 0, (0, 0)
     if pages is not None:
-        if pages.dim() != 3 or pages.shape[:2] != (n, hkv) or pages.dtype != torch.int32 or pages.shape[2] == 0:
+        if pages.dim() != 3 or pages.shape[:2] != (n, hkv) or pages.dtype is not torch.int32 or pages.shape[2] == 0:
             raise ValueError(f"{what}: pages must be int32 [{n}, {hkv}, top]")
         if pages.stride(-1) != 1:
             raise ValueError(f"{what}: pages needs a contiguous last dimension")
@@ -129,8 +130,8 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
             out = torch.empty((n, hq, d), dtype=torch.float32, device=query.device)
             m, l = torch.empty((2, n, hq), dtype=torch.float32, device=query.device).unbind(0)
     elif out is None:
-        out = torch.empty((n, hq, d), dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    elif out.shape != query.shape or out.dtype is not query.dtype or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must be [{n}, {hq}, {d}] in the cache's dtype, last dimension contiguous")
     bounds = None if select is None else select[0]
     idx = _lib.same_device(what, query, k_cache, v_cache, block_table, seq_lens, pages, out, ws, status, bounds)
@@ -140,12 +141,12 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
         need = workspace_bytes(hq, hkv, d, top * bs if top else int(max_seq_len))
         if select is not None:
             need += select_workspace_bytes(n, hkv, int(max_seq_len), bs, top)
-        ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+        ws = seq_lens.new_empty((need + 3) // 4) if need else None
     P = _lib.addr
     a = _lib.pack_paged_attn(
         query.data_ptr(), *query.stride()[:2], k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(),
         *v_cache.stride()[:3], block_table.data_ptr(), *block_table.stride(), seq_lens.data_ptr(), P(pages), *pg,
-        out.data_ptr(), *out.stride()[:2], P(m), P(l), P(status), _lib.dtype_code(query), n, hq, hkv, d, nb, bs,
+        out.data_ptr(), *out.stride()[:2], P(m), P(l), P(status), _CODES[query.dtype], n, hq, hkv, d, nb, bs,
         block_table.shape[1], int(max_seq_len), top, float(scale))
     size = 0 if ws is None else ws.nbytes
     if select is None:
@@ -178,21 +179,20 @@ def update_page_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table:
     max_new=1 after a decode step, with the longest prompt after a prefill. Other pages'
     bounds stay as they are."""
     what = "update_page_bounds"
-    _check_cache(what, k_cache, "k_cache", k_cache.dtype)
-    nb, bs, hkv, d = k_cache.shape
-    if bounds.shape != (nb, hkv, 2, d) or bounds.dtype != k_cache.dtype or bounds.stride(-1) != 1 \
+    nb, bs, hkv, d = _cache_sizes(what, "k_cache", k_cache, k_cache.dtype)
+    if bounds.shape != (nb, hkv, 2, d) or bounds.dtype is not k_cache.dtype or bounds.stride(-1) != 1 \
             or bounds.stride(-2) != d:
         raise ValueError(f"{what}: bounds must be [{nb}, {hkv}, 2, {d}] in the cache's dtype, (lo, hi) contiguous")
     n = block_table.shape[0]
-    block_table, seq_lens = _check_table(what, n, block_table, seq_lens)
+    block_table, seq_lens = _tables(what, n, block_table, seq_lens)
     if new_lens is not None:
-        if tuple(new_lens.shape) != (n,):
+        if new_lens.shape != (n,):
             raise ValueError(f"{what}: new_lens must be [{n}]")
-        new_lens = _i32(new_lens).contiguous()
+        new_lens = new_lens.to(torch.int32).contiguous()
     idx = _lib.same_device(what, k_cache, bounds, block_table, seq_lens, new_lens, status)
     a = _lib.pack_page_bounds(
         k_cache.data_ptr(), *k_cache.stride()[:3], bounds.data_ptr(), *bounds.stride()[:2], block_table.data_ptr(),
-        *block_table.stride(), seq_lens.data_ptr(), _lib.addr(new_lens), _lib.addr(status), _lib.dtype_code(k_cache),
+        *block_table.stride(), seq_lens.data_ptr(), _lib.addr(new_lens), _lib.addr(status), _CODES[k_cache.dtype],
         n, hkv, d, nb, bs, block_table.shape[1], int(max_seq_len), int(max_new))
     _lib.launch(what, idx, _lib.lib().starkv_page_bounds, a)
 
@@ -201,9 +201,9 @@ def _check_bounds(what: str, query, bounds, top, sinks, recent):
     if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.shape[3] not in HEAD_DIMS:
         raise ValueError(f"{what}: bounds must be [num_blocks, H_kv, 2, 64 or 128]")
     nb, hkv, _, d = bounds.shape
-    if bounds.dtype != query.dtype or query.dtype not in (torch.bfloat16, torch.float16):
+    if bounds.dtype is not query.dtype or query.dtype not in _CODES:
         raise ValueError(f"{what}: query and bounds must be bf16 or f16, both the same")
-    if bounds.stride(-1) != 1 or bounds.stride(-2) != d:
+    if bounds.stride(3) != 1 or bounds.stride(2) != d:
         raise ValueError(f"{what}: the (lo, hi) rows of bounds must be contiguous")
     if top < 1 or sinks < 0 or recent < 0 or sinks + recent > top:
         raise ValueError(f"{what}: need top >= 1 and sinks + recent <= top")
@@ -222,23 +222,22 @@ def select_pages(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.T
     Scores in 64 bits; ties go to the lowest page; a NaN score ranks above all others."""
     what = "select_pages"
     nb, hkv, d = _check_bounds(what, query, bounds, top, sinks, recent)
-    _check_query(what, query, hkv, d)
-    n, hq, _ = query.shape
-    block_table, seq_lens = _check_table(what, n, block_table, seq_lens)
+    n, hq, _ = _query_sizes(what, query, hkv, d)
+    block_table, seq_lens = _tables(what, n, block_table, seq_lens)
     if out is None:
-        out = torch.empty((n, hkv, top), dtype=torch.int32, device=query.device)
-    elif tuple(out.shape) != (n, hkv, top) or out.dtype != torch.int32 or out.stride(-1) != 1:
+        out = seq_lens.new_empty((n, hkv, top))
+    elif out.shape != (n, hkv, top) or out.dtype is not torch.int32 or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must be int32 [{n}, {hkv}, {top}], last dimension contiguous")
     idx = _lib.same_device(what, query, bounds, block_table, seq_lens, out, ws, status)
     if n == 0:
         return out
     if ws is None:
         need = select_workspace_bytes(n, hkv, max_seq_len, block_size, top)
-        ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+        ws = seq_lens.new_empty((need + 3) // 4) if need else None
     a = _lib.pack_select_pages(
         query.data_ptr(), *query.stride()[:2], bounds.data_ptr(), *bounds.stride()[:2], block_table.data_ptr(),
         *block_table.stride(), seq_lens.data_ptr(), out.data_ptr(), *out.stride()[:2], _lib.addr(status),
-        _lib.dtype_code(query), n, hq, hkv, d, nb, int(block_size), block_table.shape[1], int(max_seq_len), int(top),
+        _CODES[query.dtype], n, hq, hkv, d, nb, int(block_size), block_table.shape[1], int(max_seq_len), int(top),
         int(sinks), int(recent))
     _lib.launch(what, idx, _lib.lib().starkv_select_pages, a, _lib.addr(ws), 0 if ws is None else ws.nbytes)
     return out
@@ -255,7 +254,7 @@ def sparse_paged_decode(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     nb, hkv, d = _check_bounds(what, query, bounds, top, sinks, recent)
     if (nb, hkv, d) != (k_cache.shape[0], *k_cache.shape[2:]):
         raise ValueError(f"{what}: bounds and cache must have the same blocks, heads and head_dim")
-    pages = torch.empty((query.shape[0], hkv, top), dtype=torch.int32, device=query.device)
+    pages = block_table.new_empty((query.shape[0], hkv, top), dtype=torch.int32)
     out = _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, scale, pages, out, False, None, ws,
                   status, select=(bounds, int(sinks), int(recent)))
     return out, pages

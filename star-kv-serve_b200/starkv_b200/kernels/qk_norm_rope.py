@@ -13,60 +13,66 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .paged_attention import HEAD_DIMS, _check_cache
+from .paged_attention import _CODES, HEAD_DIMS, _cache_sizes
 
 _Z2, _Z3 = (0, 0), (0, 0, 0)
 
 
-def _rows(what: str, name: str, t: torch.Tensor, n: int, heads: int, d: int, dtype) -> None:
-    if t.dim() != 3 or tuple(t.shape) != (n, heads, d) or t.dtype != dtype or t.stride(-1) != 1:
-        raise ValueError(f"{what}: {name} must be [{n}, {heads}, {d}] in the query's dtype, last dimension contiguous")
+_INDEX = {torch.int32: _lib.I32, torch.int64: _lib.I64}
+_FLOAT = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+
+
+def _rows(what: str, name: str, t: torch.Tensor, sizes, dtype) -> None:
+    if t.shape != sizes or t.dtype is not dtype or t.stride(2) != 1:
+        raise ValueError(f"{what}: {name} must be {list(sizes)} in the query's dtype, last dimension contiguous")
 
 
 def _run(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping, q_weight, k_weight, eps, q_out, k_out,
          status):
-    if q.dim() != 3 or q.shape[2] not in HEAD_DIMS or q.shape[1] == 0:
-        raise ValueError(f"{what}: q must be [n, heads, 64 or 128]")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    q_sizes, dtype = q.shape, q.dtype
+    if len(q_sizes) != 3 or q_sizes[2] not in HEAD_DIMS or q_sizes[1] == 0 or q.stride(2) != 1:
+        raise ValueError(f"{what}: q must be [n, heads, 64 or 128], last dimension contiguous")
+    if dtype not in _CODES:
         raise ValueError(f"{what}: q, k and v must be bf16 or f16")
-    n, hq, d = q.shape
-    _rows(what, "q", q, n, hq, d, q.dtype)
+    n, hq, d = q_sizes
     hkv = 0
     if k is not None:
-        hkv = k.shape[1] if k.dim() == 3 else 0
-        if hkv == 0:
+        if k.dim() != 3 or k.shape[1] == 0:
             raise ValueError(f"{what}: k must be [n, KV heads, {d}]")
-        _rows(what, "k", k, n, hkv, d, q.dtype)
-    if positions.shape != (n,) or positions.dtype not in (torch.int32, torch.int64):
+        hkv = k.shape[1]
+        k_sizes = (n, hkv, d)
+        _rows(what, "k", k, k_sizes, dtype)
+    if positions.shape != (n,) or positions.dtype not in _INDEX:
         raise ValueError(f"{what}: positions must be int32 or int64 [{n}]")
-    if cos_sin_cache.dim() != 2 or cos_sin_cache.stride(-1) != 1 or cos_sin_cache.shape[1] % 16 or \
-            not 0 < cos_sin_cache.shape[1] <= d:
-        raise ValueError(f"{what}: cos_sin_cache must be [positions, rot], rot a multiple of 16 and at most {d}")
-    w_dtype = 0
+    if cos_sin_cache.dim() != 2 or cos_sin_cache.dtype not in _FLOAT:
+        raise ValueError(f"{what}: cos_sin_cache must be a bf16, f16 or f32 [positions, rot]")
+    rows, rot = cos_sin_cache.shape
+    if cos_sin_cache.stride(1) != 1 or rot % 16 or not 0 < rot <= d:
+        raise ValueError(f"{what}: cos_sin_cache must be [positions, rot], contiguous rows, rot a multiple of 16 and at "
+                         f"most {d}")
+    w_dtype = None
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None:
-            if tuple(w.shape) != (d,) or not w.is_contiguous():
-                raise ValueError(f"{what}: {name} must be a contiguous [{d}]")
-            w_dtype = _lib.dtype_code(w)
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError(f"{what}: q_weight and k_weight must share one dtype")
+            if w.shape != (d,) or w.dtype not in _FLOAT or not w.is_contiguous():
+                raise ValueError(f"{what}: {name} must be a contiguous bf16, f16 or f32 [{d}]")
+            if w_dtype not in (None, w.dtype):
+                raise ValueError(f"{what}: q_weight and k_weight must share one dtype")
+            w_dtype = w.dtype
     nb = bs = slot_dtype = 0
     if k_cache is not None:
-        _check_cache(what, k_cache, "k_cache", q.dtype)
-        _check_cache(what, v_cache, "v_cache", q.dtype)
-        if k_cache.shape != v_cache.shape or k_cache.shape[2:] != (hkv, d):
+        nb, bs = _cache_sizes(what, "k_cache", k_cache, dtype)[:2]
+        if _cache_sizes(what, "v_cache", v_cache, dtype) != k_cache.shape or k_cache.shape[2:] != (hkv, d):
             raise ValueError(f"{what}: k_cache and v_cache must both be [num_blocks, block_size, {hkv}, {d}]")
-        _rows(what, "v", v, n, hkv, d, q.dtype)
-        if slot_mapping.shape != (n,) or slot_mapping.dtype not in (torch.int32, torch.int64):
+        _rows(what, "v", v, k_sizes, dtype)
+        if slot_mapping.shape != (n,) or slot_mapping.dtype not in _INDEX:
             raise ValueError(f"{what}: slot_mapping must be int32 or int64 [{n}]")
-        nb, bs = k_cache.shape[:2]
-        slot_mapping, slot_dtype = slot_mapping.contiguous(), _lib.dtype_code(slot_mapping)
+        slot_mapping, slot_dtype = slot_mapping.contiguous(), _INDEX[slot_mapping.dtype]
     if q_out is None:
-        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _rows(what, "q_out", q_out, n, hq, d, q.dtype)
+        _rows(what, "q_out", q_out, q_sizes, dtype)
     if k_out is not None:
-        _rows(what, "k_out", k_out, n, hkv, d, q.dtype)
+        _rows(what, "k_out", k_out, k_sizes, dtype)
     positions = positions.contiguous()
     idx = _lib.same_device(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping, q_weight, k_weight,
                            q_out, k_out, status)
@@ -78,9 +84,9 @@ def _run(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping
         P(v), *(_Z2 if v is None else v.stride()[:2]), q_out.data_ptr(), *q_out.stride()[:2],
         P(k_out), *(_Z2 if k_out is None else k_out.stride()[:2]), P(q_weight), P(k_weight), positions.data_ptr(),
         cos_sin_cache.data_ptr(), cos_sin_cache.stride(0), P(k_cache), *(_Z3 if k_cache is None else k_cache.stride()[:3]),
-        P(v_cache), *(_Z3 if v_cache is None else v_cache.stride()[:3]), P(slot_mapping), P(status), _lib.dtype_code(q),
-        w_dtype, _lib.dtype_code(positions), _lib.dtype_code(cos_sin_cache), slot_dtype, n, hq, hkv, d,
-        cos_sin_cache.shape[1], cos_sin_cache.shape[0], nb, bs, float(eps))
+        P(v_cache), *(_Z3 if v_cache is None else v_cache.stride()[:3]), P(slot_mapping), P(status), _CODES[dtype],
+        _FLOAT.get(w_dtype, 0), _INDEX[positions.dtype], _FLOAT[cos_sin_cache.dtype], slot_dtype, n, hq, hkv, d, rot,
+        rows, nb, bs, float(eps))
     _lib.launch(what, idx, _lib.lib().starkv_norm_rope, a)
     return q_out
 
@@ -95,7 +101,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if k is None and (k_out is not None or k_weight is not None):
         raise ValueError("qk_norm_rope: k_out and k_weight need k")
     if k is not None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     q_out = _run("qk_norm_rope", q, k, None, positions, cos_sin_cache, None, None, None, q_weight, k_weight, eps, q_out,
                  k_out, status)
     return q_out, k_out
