@@ -764,7 +764,7 @@ int starkv_norm_rope(const StarKVNormRopeArgs* a, void* stream) {
   p.n = a->n; p.num_heads = a->num_heads; p.num_kv_heads = a->num_kv_heads; p.status = a->status;
   DeviceInfo dev;
   if (const int st = device_info(dev)) return st;
-  return launch_norm_rope(p, a->dtype, a->head_dim, (cudaStream_t)stream);
+  return launch_norm_rope(p, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream);
 }
 
 int starkv_read_status(void* workspace, int32_t* host_status, int32_t reset, void* stream) {

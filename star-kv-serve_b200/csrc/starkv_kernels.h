@@ -228,7 +228,7 @@ size_t paged_attn_workspace_bytes(int rows, int head_dim, int max_tokens);
 int launch_paged_attn(const PagedAttnParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
 int launch_page_bounds(const PageBoundsParams& p, int dtype, int head_dim, cudaStream_t stream);
 int launch_select_pages(SelectPagesParams p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
-int launch_norm_rope(const NormRopeParams& p, int dtype, int head_dim, cudaStream_t stream);
+int launch_norm_rope(const NormRopeParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
 int launch_prefill(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PrefillParams& p,
                    int q_tiles, cudaStream_t stream);
 
