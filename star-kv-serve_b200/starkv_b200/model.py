@@ -5,7 +5,10 @@ residual, final RMSNorm, LM head logits.
 Compressed layers run starkv_b200.layer.StarKVAttentionLayer (this library's paged
 low-rank decode); the layers the checkpoint left full-rank run stock attention
 over a paged bf16 K/V cache (vLLM's paged-attention and cache-write ops, as the
-reference's stock LlamaAttention does). Tensor parallel over `world` ranks in the
+reference's stock LlamaAttention does), or with full_attention="paged" this library's
+own full-rank layer (starkv_b200.full_layer: per-head norms where cfg.qk_norm says so,
+decode over selected pages with full_top_pages, pages split over the ranks with
+attn_parallel="context"). Tensor parallel over `world` ranks in the
 Megatron layout the reference leaves at TP=1 (model.py:32-33): attention heads and
 the MLP's intermediate columns are split, o_proj and down_proj are row-parallel
 and all-reduced; embedding, norms and LM head are replicated. Weights are
@@ -29,6 +32,7 @@ import torch.nn.functional as F
 
 from . import sharding
 from .collectives import all_reduce_
+from .full_layer import FullAttentionLayer, FullContextLayer
 from .layer import HEAD_DIM, AttnWeights, StarKVAttentionLayer, StarKVContextLayer, rope
 from .workload import rope_cos_sin
 
@@ -44,6 +48,7 @@ class ModelConfig:
     rms_eps: float = 1e-5
     max_pos: int = 32768
     seed: int = 0
+    qk_norm: bool = False                # full-rank layers norm each query and key head (full_attention="paged")
     k_rank_choices: tuple = (16, 32, 48)         # comp-ratio 0.75: W ~ 1000 for 32 heads
     k_rank_probs: tuple = (0.35, 0.45, 0.20)
     v_rank_choices: tuple = (32, 64)             # rv ~ 1280
@@ -123,8 +128,14 @@ class StarKVModel:
     """The model on one rank of a tensor-parallel group (world 1: whole)."""
 
     def __init__(self, cfg: ModelConfig, device, quant: bool = False, rank: int = 0, world: int = 1, group=None,
-                 dtype=torch.bfloat16, attn_parallel: str = "heads", checkpoint=None):
-        """`checkpoint`: a fused_weights.pt (path, state dict or loaded
+                 dtype=torch.bfloat16, attn_parallel: str = "heads", checkpoint=None, full_attention: str = "stock",
+                 full_top_pages: int | None = None):
+        """`full_attention`: "stock" (vLLM's ops) or "paged" (this library's kernels) for
+        the full-rank layers; `full_top_pages` lets the latter decode over that many pages
+        per sequence and KV head. With attn_parallel="context" "paged" layers split their
+        pages over the ranks as the compressed layers do.
+
+        `checkpoint`: a fused_weights.pt (path, state dict or loaded
         starkv_b200.checkpoint.StarKVCheckpoint) whose compressed layers' K/V factors
         the model serves; the layers it leaves out are full-rank. Without one, every
         layer outside cfg.full_layers gets seeded random factors. The other weights
@@ -132,6 +143,12 @@ class StarKVModel:
         either way: the checkpoint holds only the K/V factors."""
         if attn_parallel not in ("heads", "context"):
             raise ValueError(f"attn_parallel must be 'heads' or 'context', not {attn_parallel!r}")
+        if full_attention not in ("stock", "paged"):
+            raise ValueError(f"full_attention must be 'stock' or 'paged', not {full_attention!r}")
+        if full_attention == "stock" and (full_top_pages is not None or cfg.qk_norm):
+            raise ValueError("full_top_pages and qk_norm need full_attention='paged'")
+        if full_top_pages is not None and attn_parallel == "context":
+            raise ValueError("full_top_pages: pages are selected over a whole sequence, not over a rank's share")
         ckpt = None
         if checkpoint is not None:
             import dataclasses
@@ -142,7 +159,7 @@ class StarKVModel:
                 raise ValueError("checkpoint loaded with kv_quant != the model's quant")
             cfg = dataclasses.replace(cfg, full_layers=tuple(ckpt.skip_layers))
         self.cfg, self.quant, self.rank, self.world, self.group = cfg, quant, rank, world, group
-        self.attn_parallel = attn_parallel
+        self.attn_parallel, self.full_attention = attn_parallel, full_attention
         self.device = torch.device(device)
         d, H = cfg.hidden, cfg.heads
         g = torch.Generator(device=self.device).manual_seed(cfg.seed)
@@ -162,7 +179,15 @@ class StarKVModel:
             if i in cfg.full_layers:
                 wk = _rnd((H * HEAD_DIM, d), d ** -0.5, gl, self.device, dtype)
                 wv = _rnd((H * HEAD_DIM, d), d ** -0.5, gl, self.device, dtype)
-                attn = StockAttentionLayer(wq, wk, wv, wo, self.cos_sin_cache, rank, world, group)
+                if full_attention == "stock":
+                    attn = StockAttentionLayer(wq, wk, wv, wo, self.cos_sin_cache, rank, world, group)
+                else:
+                    norm = torch.ones(HEAD_DIM, device=self.device, dtype=dtype) if cfg.qk_norm else None
+                    kw = dict(rank=rank, world=world, group=group, q_norm=norm, k_norm=norm, eps=cfg.rms_eps)
+                    if attn_parallel == "context":
+                        attn = FullContextLayer(wq, wk, wv, wo, self.cos_sin_cache, **kw)
+                    else:
+                        attn = FullAttentionLayer(wq, wk, wv, wo, self.cos_sin_cache, top_pages=full_top_pages, **kw)
                 del wk, wv
             elif ckpt is not None:
                 w = AttnWeights.from_checkpoint(ckpt.layers[i], wq, wo, H, device=self.device, dtype=dtype)
@@ -201,12 +226,15 @@ class StarKVModel:
     def allocate_caches(self, num_blocks: int, compressed_blocks: int | None = None) -> list:
         """One paged cache per layer (16-token blocks): STAR-KV code rows
         (`compressed_blocks` of them, default `num_blocks`: with attn_parallel
-        "context" a rank holds only its pages of every sequence), or the stock
-        (key, value) pair."""
+        "context" a rank holds only its pages of every sequence), or the (key, value)
+        pair of a full-rank layer (with page bounds where it selects pages)."""
         caches = []
         for ly in self.layers:
             a = ly["attn"]
-            if ly["full"]:
+            if isinstance(a, FullAttentionLayer):
+                split = isinstance(a, FullContextLayer) and compressed_blocks is not None
+                caches.append(a.allocate_cache(compressed_blocks if split else num_blocks))
+            elif ly["full"]:
                 ks, vs = a.cache_shapes(num_blocks)
                 caches.append((torch.zeros(ks, dtype=torch.bfloat16, device=self.device),
                                torch.zeros(vs, dtype=torch.bfloat16, device=self.device)))
@@ -221,7 +249,9 @@ class StarKVModel:
         tot = 0.0
         for ly in self.layers:
             a = ly["attn"]
-            if ly["full"]:
+            if isinstance(a, FullAttentionLayer):
+                tot += a.bytes_per_token()
+            elif ly["full"]:
                 tot += 2 * a.heads * HEAD_DIM * 2
             else:
                 width, dt = a.cache_row()
@@ -249,7 +279,11 @@ class StarKVModel:
         x = self.embed[tokens]
         for ly, cache in zip(self.layers, caches):
             h = rms_norm(x, ly["norms"][0], eps)
-            if ly["full"]:
+            if isinstance(ly["attn"], FullAttentionLayer):
+                meta = cmeta if isinstance(ly["attn"], FullContextLayer) else (block_table, seq_lens, max_seq_len,
+                                                                               slot_mapping)
+                a = ly["attn"].forward(h, positions, cache, *meta)
+            elif ly["full"]:
                 a = ly["attn"].forward(h, positions, cache[0], cache[1], block_table, seq_lens, max_seq_len,
                                        slot_mapping)
             else:

@@ -161,3 +161,28 @@ def test_c_entry_points_refuse_before_any_gpu_work():
     assert call("select", sinks=3) == call("select", top=0) == call("select", recent=-1) == 22
     assert call("select") == 102
     assert call("select", ws=(A + 4, 1 << 20)) == 100
+
+
+def test_full_layer_and_model_refusals():
+    from starkv_b200.full_layer import FullAttentionLayer
+    from starkv_b200.model import ModelConfig, StarKVModel
+    w = lambda h: torch.zeros(h * 128, 64, dtype=BF)  # noqa: E731
+    wo, cs = torch.zeros(64, 6 * 128, dtype=BF), torch.zeros(8, 128, dtype=BF)
+    one = torch.ones(128, dtype=BF)
+    for kw, say in ((dict(world=2), "split over 2"), (dict(q_norm=one), "both"), (dict(top_pages=1), "at least 2")):
+        with pytest.raises(ValueError, match=say):
+            FullAttentionLayer(w(6), w(3), w(3), wo, cs, **kw)
+    with pytest.raises(ValueError, match="do not group"):
+        FullAttentionLayer(w(6), w(4), w(4), wo, cs)
+    layer = FullAttentionLayer(w(6), w(3), w(3), wo, cs, top_pages=4)
+    assert layer.bytes_per_token() == (2 + 2 / 16) * 3 * 256
+    with pytest.raises(ValueError, match="cover"):
+        layer.prefill(torch.zeros(3, 64, dtype=BF), None, [2], None, None)
+    with pytest.raises(ValueError, match="block_table"):
+        layer.prefill(torch.zeros(3, 64, dtype=BF), None, [3], None, None)
+    for kw, say in ((dict(full_attention="flash"), "stock"), (dict(full_top_pages=4), "need full_attention"),
+                    (dict(full_attention="paged", full_top_pages=4, attn_parallel="context"), "whole sequence")):
+        with pytest.raises(ValueError, match=say):
+            StarKVModel(ModelConfig(layers=1), "cpu", **kw)
+    with pytest.raises(ValueError, match="qk_norm"):
+        StarKVModel(ModelConfig(layers=1, qk_norm=True), "cpu")
