@@ -640,12 +640,12 @@ int starkv_page_bounds(const StarKVPageBoundsArgs* a, void* stream) {
   return launch_page_bounds(p, a->dtype, a->head_dim, (cudaStream_t)stream);
 }
 
-// 8 bytes of score per page of the longest sequence, (sequence and) KV head
+// order keys of the scores, per page of the longest sequence, sequence and KV head
 size_t starkv_select_pages_workspace_bytes(int32_t n, int32_t num_kv_heads, int32_t max_tokens, int32_t block_size,
                                            int32_t top) {
   if (n <= 0 || num_kv_heads <= 0 || max_tokens <= 0 || block_size <= 0) return 0;
   const size_t pages = ((size_t)max_tokens + block_size - 1) / block_size;
-  return pages <= (size_t)std::max(top, 0) ? 0 : (pages * n * num_kv_heads * 8 + 255) / 256 * 256;
+  return pages <= (size_t)std::max(top, 0) ? 0 : (starkv::select_scratch_bytes((int64_t)n * num_kv_heads, pages) + 255) / 256 * 256;
 }
 
 static int select_pages_params(const StarKVSelectPagesArgs* a, void* workspace, size_t workspace_bytes,
@@ -675,7 +675,7 @@ static int select_pages_params(const StarKVSelectPagesArgs* a, void* workspace, 
   const size_t need = starkv_select_pages_workspace_bytes(a->n, a->num_kv_heads, max_len, a->block_size, a->top);
   if (need && (!workspace || workspace_bytes < need)) return STARKV_EWORKSPACE;
   if (need && (reinterpret_cast<uintptr_t>(workspace) & 15)) return STARKV_EALIGN;
-  p.keys = reinterpret_cast<uint64_t*>(workspace);
+  p.scratch = workspace;
   p.key_stride = ((int64_t)max_len + a->block_size - 1) / a->block_size;
   return STARKV_OK;
 }

@@ -126,7 +126,7 @@ constexpr float weight_bias() {
 __device__ __forceinline__ int unit_tokens(const PagedAttnParams& p, int b) {
   const int L = min(max(p.seq_lens[b], 0), p.max_len);
   if (!p.pages) return L;
-  return min(p.top, (L + p.block_size - 1) / p.block_size) * p.block_size;
+  return min(p.top, (int)(((unsigned)L + (unsigned)p.block_size - 1u) / (unsigned)p.block_size)) * p.block_size;
 }
 // Work items (runs of 2^item_shift tokens) of a unit of sequence b.
 __device__ __forceinline__ int unit_items(const PagedAttnParams& p, int b) {

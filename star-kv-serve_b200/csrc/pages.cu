@@ -9,16 +9,20 @@
 //               = sum_d up[d] hi[d] + down[d] lo[d],
 //   up = sum_g max(q[g], 0),  down = sum_g min(q[g], 0),
 // an upper bound of sum_g q[g] . k over the page's keys. One page costs 4 D bytes and 2 D
-// multiply-adds whatever G is, so the read of the bounds is the cost. Scores are summed
-// in 64 bits: the products of two 16-bit values are exact there and the order of two
-// pages next to the border does not depend on how the sum was split (32-bit sums put
-// about one of a thousand selections on the other side).
+// multiply-adds whatever G is, so the read of the bounds is the cost.
 //
-// score_kernel takes the batch's pages in runs of 32, an equal number of runs per warp
-// whatever the mix of lengths, and writes order-preserving 64-bit keys. pick_kernel takes
-// a CTA per (sequence, KV head) and finds the border by radix selection from the highest
-// bit in which the unit's keys differ (one or two passes of 8 bits on real scores). Ties
-// go to the lowest page.
+// The selection is that of scores summed in 64 bits (products of two 16-bit values are
+// exact there, so the order of two pages next to the border does not depend on how a sum
+// is split; 32-bit sums put about one of a thousand selections on the other side). 64-bit
+// conversions run at an eighth of the rate that the reads need, so score_kernel sums in
+// f32 and also bounds the error, and pick_kernel sums again in 64 bits only the pages
+// that lie within the error of the border, mostly none.
+//
+// score_kernel takes the batch's pages in runs of 16, an equal number of runs per warp
+// whatever the mix of lengths, and writes order-preserving keys. pick_kernel takes a CTA
+// per (sequence, KV head) and finds the border by radix selection from the highest bit in
+// which the unit's keys differ (one or two passes of 8 bits on real scores). Ties go to
+// the lowest page.
 #include <algorithm>
 #include <type_traits>
 
@@ -110,24 +114,68 @@ __global__ void __launch_bounds__(kThreads) bounds_kernel(const PageBoundsParams
   if (sub == 1) *reinterpret_cast<uint4*>(out + D) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
 }
 
-// Order of doubles as order of unsigned integers; -0 as +0, every NaN above all numbers.
+// Order of numbers as order of unsigned integers; -0 as +0, every NaN above all numbers.
 __device__ __forceinline__ uint64_t order_key(double x) {
   if (x != x) return ~0ull;
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
   return u >> 63 ? ~u : u | (1ull << 63);
+}
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return ~0u;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u >> 31 ? ~u : u | (1u << 31);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&d))
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)),
+        "l"(*reinterpret_cast<const uint64_t*>(&c)));
+  return d;
+}
+
+// The larger magnitude of two pairs (its sign means nothing); a NaN loses.
+__device__ __forceinline__ uint32_t max_abs2(__nv_bfloat16, uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t max_abs2(__half, uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// up (upper) or down of channels d .. d + 7 of a KV head's queries
+template <typename T, typename W>
+__device__ __forceinline__ void query_side(const T* q, int64_t stride, int group, bool upper, W (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 0;
+#pragma unroll 4
+  for (int h = 0; h < group; ++h) {
+    float f[8];
+    to_f32x8(T{}, *reinterpret_cast<const uint4*>(q + h * stride), f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] += (W)(upper ? (f[i] < 0.f ? 0.f : f[i]) : (f[i] > 0.f ? 0.f : f[i]));
+  }
 }
 
 // Pages of sequence b, and how many of them compete: all but the kept ones, none where
 // every page is taken.
 __device__ __forceinline__ int pages_of(const SelectPagesParams& p, int b) {
   const int L = min(max(p.seq_lens[b], 0), p.max_len);
-  return (int)(((int64_t)L + p.block_size - 1) / p.block_size);
+  return (int)(((unsigned)L + (unsigned)p.block_size - 1u) / (unsigned)p.block_size);   // L <= 2^30
 }
 __device__ __forceinline__ int competing(const SelectPagesParams& p, int pages) {
   return pages <= p.top || p.sinks + p.recent == p.top ? 0 : pages - p.sinks - p.recent;
 }
 
-constexpr int kRun = 32;     // pages of a run
+constexpr int kRun = 16;     // pages of a run
+constexpr int kBatch = 32;   // block ids that a warp holds
 constexpr int kStep = 4;     // pages of a lane's step
 constexpr int kRing = 3;     // steps in the copies' ring
 constexpr int kRingBytes = kRing * kStep * 16 * kThreads;
@@ -137,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
   extern __shared__ __align__(16) uint8_t ring[];
   constexpr int LP = 2 * D / 8;                      // lanes of one page's bounds
   constexpr int kPer = kStep * (32 / LP);            // pages of a warp's step
-  constexpr int kSteps = kRun / kPer;                // steps of a run
+  constexpr int kSteps = kBatch / kPer;              // steps of a batch of block ids
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int e = lane % LP, sub = lane / LP;
   const int d = (e * 8) % D;
@@ -166,8 +214,7 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
     // two steps ahead): no barrier between copy and use. Block ids come 32 at a time.
     const uint32_t slots = smem_u32(ring) + tid * 16;
     auto blocks_from = [&](int i) {   // lane l: the block of competing page i + l
-      if (i + lane >= i1) return 0;
-      int blk = bt[(int64_t)(i + lane) * p.bt_s1];
+      int blk = bt[(int64_t)min(i + lane, i1 - 1) * p.bt_s1];   // past the end: the last page once more
       if ((unsigned)blk >= (unsigned)p.num_blocks) {
         record_status(p.status, STARKV_EBOUNDS);
         blk = 0;
@@ -178,43 +225,43 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
     auto issue = [&](int j) {
       if (j % kSteps == 0) {
         cur = nxt;
-        nxt = blocks_from(i0 + (j / kSteps + 1) * kRun);
+        nxt = blocks_from(i0 + (j / kSteps + 1) * kBatch);
       }
 #pragma unroll
       for (int u = 0; u < kStep; ++u) {
-        const int blk = __shfl_sync(~0u, cur, j % kSteps * kPer + sub * kStep + u);   // a page past the end: block 0
+        const int blk = __shfl_sync(~0u, cur, j % kSteps * kPer + sub * kStep + u);
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + (j % kRing * kStep + u) * kThreads * 16),
                      "l"(bounds + (int64_t)blk * p.b_s0)
                      : "memory");
       }
     };
+    // the queries before the copies, so that they do not wait behind them
+    float w[8];
+    query_side(reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group) * p.q_s1 + d, p.q_s1, p.group,
+               upper, w);
+    float size = 0.f;                                // sum of |w| of this lane's channels
+#pragma unroll
+    for (int i = 0; i < 8; ++i) size += fabsf(w[i]);
     issue(0);
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (steps > 1) issue(1);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    double w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 0.0;
-    const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group) * p.q_s1 + d;
-#pragma unroll 4
-    for (int h = 0; h < p.group; ++h) {
-      float f[8];
-      to_f32x8(T{}, *reinterpret_cast<const uint4*>(q + h * p.q_s1), f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] += (double)(upper ? (f[i] < 0.f ? 0.f : f[i]) : (f[i] > 0.f ? 0.f : f[i]));
-    }
-    uint64_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride + i0;
+    uint32_t k_lo = ~0u, k_hi = 0;
+    uint32_t largest = 0;                            // largest |bound| of this lane's channels, as a pair
+    uint32_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride + i0;
     for (int j = 0; j < steps; ++j) {
       asm volatile("cp.async.wait_group 1;" ::: "memory");
-      double s[kStep];
+      float s[kStep];
 #pragma unroll
       for (int u = 0; u < kStep; ++u) {
         const uint4 v = *reinterpret_cast<const uint4*>(ring + ((j % kRing * kStep + u) * kThreads + tid) * 16);
         float f[8];
         to_f32x8(T{}, v, f);
-        s[u] = 0.0;
+        float2 a = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[u] = fma((double)f[i], w[i], s[u]);
+        for (int i = 0; i < 4; ++i) a = fma2(make_float2(f[2 * i], f[2 * i + 1]), make_float2(w[2 * i], w[2 * i + 1]), a);
+        s[u] = a.x + a.y;
+        largest = max_abs2(T{}, max_abs2(T{}, max_abs2(T{}, largest, v.x), v.y), max_abs2(T{}, v.z, v.w));
       }
       if (j + 2 < steps) issue(j + 2);   // into the slots of step j - 1
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -224,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
       for (int h = kStep / 2; h >= 1; h >>= 1, o >>= 1) {
 #pragma unroll
         for (int i = 0; i < h; ++i) {
-          const double give = lane & o ? s[i] : s[i + h], keep = lane & o ? s[i + h] : s[i];
+          const float give = lane & o ? s[i] : s[i + h], keep = lane & o ? s[i + h] : s[i];
           s[i] = keep + __shfl_xor_sync(~0u, give, o);
         }
         at += lane & o ? h : 0;
@@ -232,8 +279,30 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
       const int last = o;                            // lanes below: copies of the same page
 #pragma unroll
       for (; o; o >>= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
-      if ((lane & (2 * last - 1)) == 0 && i0 + at < i1) keys[at] = order_key(s[0]);
+      if ((lane & (2 * last - 1)) == 0 && i0 + at < i1) {
+        const uint32_t k = order_key(s[0]);
+        keys[at] = k;
+        k_lo = min(k_lo, k);
+        k_hi = max(k_hi, k);
+      }
     }
+    // Error of these scores: a term passes at most G - 1 roundings of 2^-24 in its weight
+    // (of terms of one sign), 5 in the lane and 5 between lanes, so (G + 9) 2^-24
+    // sum |w b| <= (G + 9) 2^-24 sum_lanes largest * size; 1.125 times (G + 11) covers the
+    // roundings of the bound itself.
+    float err;
+    {
+      float f[8];
+      to_f32x8(T{}, make_uint4(largest, 0, 0, 0), f);
+      err = fmaxf(fabsf(f[0]), fabsf(f[1])) * size;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) err += __shfl_xor_sync(~0u, err, o);   // D = 64: both halves, an upper bound
+      err *= 1.125f / (1 << 24) * (p.group + 11);
+    }
+    k_lo = __reduce_min_sync(~0u, k_lo);
+    k_hi = __reduce_max_sync(~0u, k_hi);
+    uint4* about = p.runs + ((int64_t)b * p.num_kv_heads + hk) * p.run_stride + run;
+    for (int r = lane; r < here; r += 32) about[r] = make_uint4(__float_as_uint(err), k_lo, k_hi, 0);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     g += here;
     run = 0;
@@ -247,13 +316,150 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
   }
 }
 
-constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
+constexpr int kPickWarpsMost = 32;
+constexpr int kAhead = 4;         // keys in flight per thread
+constexpr int kPickCache = 8192;  // keys that are copied to shared memory
 
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectPagesParams p) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint64_t warp_lo[kPickWarps], warp_hi[kPickWarps];
-  __shared__ uint32_t scan[8], found[3];             // bin, still needed in it, its count
-  __shared__ int n_gt[kPickWarps], n_eq[kPickWarps];
+constexpr int kBins = 2048;
+constexpr int kNear = 256;        // pages next to the border that are scored again one by one
+
+struct PickShared {
+  union {
+    uint32_t hist[256];
+    uint4 bins[kBins / 4];
+  };
+  uint64_t lo[kPickWarpsMost], hi[kPickWarpsMost];
+  uint32_t scan[8], found[3];                 // bin, still needed in it, its count
+  uint32_t sure[256], tied[256];                     // 32 pages a word
+  int gt[8], eq[8];
+  int above, near;
+  uint32_t in, off;
+  int near_page[kNear];
+  uint64_t near_key[kNear];
+  double side[256];                                  // query_side of the 2 D channels of a page's bounds
+};
+
+// The border of the `rest` largest of N > rest keys, all between k_lo and k_hi: those with
+// key >> shift > border and, lowest index first, `rest` (as it comes back) of the `level`
+// ones with key >> shift == border.
+template <int kThr, typename K>
+__device__ void find_border(const K* keys, int N, K k_lo, K k_hi, PickShared& sh, int& shift, K& border, int& rest,
+                            int& level) {
+  constexpr int kBits = sizeof(K) * 8;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < 256) sh.hist[tid] = 0;
+  __syncthreads();
+  const int top_bit = k_lo == k_hi ? -1 : 63 - __clzll((long long)(k_lo ^ k_hi));
+  shift = top_bit + 1;                               // bits above are the same in all keys
+  border = shift >= kBits ? 0 : k_lo >> shift;
+  level = N;
+  while (shift > 0) {
+    const int bits = min(8, shift), ns = shift - bits;
+    for (int i = tid; i < N; i += kAhead * kThr) {
+      K k[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) k[u] = keys[min(i + u * kThr, N - 1)];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u * kThr < N && (shift >= kBits || (k[u] >> shift) == border))
+          atomicAdd(&sh.hist[(uint32_t)(k[u] >> ns) & ((1u << bits) - 1)], 1u);
+    }
+    __syncthreads();
+    // bins from the highest down: thread t < 256 has bin 255 - t
+    uint32_t mine = 0, incl = 0;
+    if (warp < 8) {
+      mine = incl = sh.hist[255 - tid];
+      sh.hist[255 - tid] = 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(~0u, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) sh.scan[warp] = incl;
+    }
+    __syncthreads();
+    if (warp < 8) {
+      for (int w = 0; w < warp; ++w) incl += sh.scan[w];
+      if (incl >= (uint32_t)rest && incl - mine < (uint32_t)rest) {
+        sh.found[0] = 255 - (uint32_t)tid;
+        sh.found[1] = (uint32_t)rest - (incl - mine);
+        sh.found[2] = mine;
+      }
+    }
+    __syncthreads();
+    border = (K)(border << bits) | (K)sh.found[0];
+    rest = (int)sh.found[1];
+    level = (int)sh.found[2];
+    shift = ns;
+    if (level == rest) break;                        // the whole bin is selected
+  }
+  __syncthreads();                                   // sh may be written again
+}
+
+// Writes the selected ones of N pages in ascending order, as base + index. cls(i): 1 for a
+// selected page, 2 for one of those of which the first `rest` are selected, else 0. All
+// threads; 8192 pages a round: a bit per page by ballots, then a thread per 32 pages.
+template <int kThr, class Cls>
+__device__ void write_selected(int N, PickShared& sh, const Cls& cls, int rest, int32_t* out, int base) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int gt0 = 0, eq0 = 0;                              // of the rounds before
+  for (int r0 = 0; r0 < N; r0 += 32 * 256) {
+    const int words = min(256, (N - r0 + 31) / 32);
+#pragma unroll 4
+    for (int w = warp; w < words; w += kThr / 32) {
+      const int i = r0 + w * 32 + lane;
+      const int c = i < N ? cls(i) : 0;
+      const uint32_t g = __ballot_sync(~0u, c == 1), e = __ballot_sync(~0u, c == 2);
+      if (lane == 0) {
+        sh.sure[w] = g;
+        sh.tied[w] = e;
+      }
+    }
+    __syncthreads();
+    uint32_t g = tid < words ? sh.sure[tid] : 0, e = tid < words ? sh.tied[tid] : 0;
+    int gt = __popc(g), eq = __popc(e);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, gt, o), y = __shfl_up_sync(~0u, eq, o);
+      if (lane >= o) {
+        gt += x;
+        eq += y;
+      }
+    }
+    if (lane == 31 && warp < 8) {
+      sh.gt[warp] = gt;
+      sh.eq[warp] = eq;
+    }
+    __syncthreads();
+    int gt_all = 0, eq_all = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) {
+        gt += sh.gt[w];
+        eq += sh.eq[w];
+      }
+      gt_all += sh.gt[w];
+      eq_all += sh.eq[w];
+    }
+    gt += gt0 - __popc(g);                           // before this thread's pages
+    eq += eq0 - __popc(e);
+    for (uint32_t m = g | e; m; m &= m - 1) {
+      const uint32_t bit = m & -m;
+      if (g & bit) out[gt++ + min(eq, rest)] = base + r0 + tid * 32 + __ffs(bit) - 1;
+      else if (eq++ < rest) out[gt + eq - 1] = base + r0 + tid * 32 + __ffs(bit) - 1;
+    }
+    gt0 += gt_all;
+    eq0 += eq_all;
+    __syncthreads();
+  }
+}
+
+// kThr: 256 threads where the units fill the GPU (four CTAs to an SM), 1024 where they do
+// not and a unit's passes over many keys are the time (8192 pages: 20.9 -> 13.2 us).
+template <typename T, int D, int kThr>
+__global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPagesParams p) {
+  __shared__ PickShared sh;
+  __shared__ uint32_t cache[kPickCache];
   const int unit = blockIdx.x;
   const int hk = unit % p.num_kv_heads, b = unit / p.num_kv_heads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -262,129 +468,287 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectPagesPar
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int32_t* out = p.pages + b * p.pg_s0 + hk * p.pg_s1;
   if (P <= p.top) {   // every page, then -1
-    for (int i = tid; i < p.top; i += kPickThreads) out[i] = i < P ? i : -1;
+    for (int i = tid; i < p.top; i += kThr) out[i] = i < P ? i : -1;
   } else {
-    for (int i = tid; i < p.sinks; i += kPickThreads) out[i] = i;
-    for (int i = tid; i < p.recent; i += kPickThreads) out[p.top - p.recent + i] = P - p.recent + i;
+    for (int i = tid; i < p.sinks; i += kThr) out[i] = i;
+    for (int i = tid; i < p.recent; i += kThr) out[p.top - p.recent + i] = P - p.recent + i;
   }
+  constexpr int LP = 2 * D / 8;
+  if (N > 0 && warp == 0) {   // for the scores in 64 bits, should there be any: before the wait it costs nothing
+    const int d = (lane % LP * 8) % D;
+    double w[8];
+    query_side(reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group) * p.q_s1 + d, p.q_s1, p.group,
+               lane % LP * 8 >= D, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sh.side[lane % LP * 8 + i] = w[i];
+  }
+  for (int i = tid; i < kBins / 4; i += kThr) sh.bins[i] = make_uint4(0, 0, 0, 0);
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the scores are written
   if (N == 0) return;
-  const uint64_t* keys = p.keys + (int64_t)unit * p.key_stride;
-  constexpr int kAhead = 4;                          // keys in flight per thread
+  out += p.sinks;
 
-  uint64_t k_lo = ~0ull, k_hi = 0;
-  for (int i = tid; i < N; i += kAhead * kPickThreads) {
+  // what the runs say: the largest error, smallest and largest key
+  uint32_t* keys = p.keys + (int64_t)unit * p.key_stride;
+  const uint4* runs = p.runs + (int64_t)unit * p.run_stride;
+  const int n_runs = (N + kRun - 1) / kRun;
+  uint32_t k_lo = ~0u, k_hi = 0, e_bits = 0;
+  uint4 about = runs[min(tid, n_runs - 1)];
+  if (N <= kPickCache) {
+    for (int i = tid; i < N; i += 2 * kAhead * kThr) {
+      uint32_t k[2 * kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const uint64_t k = keys[min(i + u * kPickThreads, N - 1)];
-      k_lo = min(k_lo, k);
-      k_hi = max(k_hi, k);
+      for (int u = 0; u < 2 * kAhead; ++u) k[u] = keys[min(i + u * kThr, N - 1)];
+#pragma unroll
+      for (int u = 0; u < 2 * kAhead; ++u)
+        if (i + u * kThr < N) cache[i + u * kThr] = k[u];
+    }
+    keys = cache;
+  }
+  for (int r = tid;;) {
+    e_bits = max(e_bits, about.x & 0x7fffffffu);     // >= 0 or NaN: ordered as integers
+    k_lo = min(k_lo, about.y);
+    k_hi = max(k_hi, about.z);
+    if ((r += kThr) >= n_runs) break;
+    about = runs[r];
+  }
+  e_bits = __reduce_max_sync(~0u, e_bits);
+  k_lo = __reduce_min_sync(~0u, k_lo);
+  k_hi = __reduce_max_sync(~0u, k_hi);
+  if (lane == 0) {
+    sh.lo[warp] = (uint64_t)k_lo << 32 | e_bits;
+    sh.hi[warp] = k_hi;
+  }
+  if (tid == 0) {
+    sh.above = sh.near = 0;
+    sh.in = ~0u;
+    sh.off = 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThr / 32; ++w) {
+    e_bits = max(e_bits, (uint32_t)sh.lo[w]);
+    k_lo = min(k_lo, (uint32_t)(sh.lo[w] >> 32));
+    k_hi = max(k_hi, (uint32_t)sh.hi[w]);
+  }
+  const int need = p.top - p.sinks - p.recent;       // < N
+  const float err = __uint_as_float(e_bits), reach = 2.01f * err;
+
+  const int e = lane % LP;
+  const int32_t* bt = p.block_table + b * p.bt_s0 + (int64_t)p.sinks * p.bt_s1;
+  const T* bounds = reinterpret_cast<const T*>(p.bounds) + (int64_t)hk * p.b_s1 + e * 8;
+  const auto score = [&](int i) {                    // in 64 bits, by a whole warp
+    int blk = bt[(int64_t)i * p.bt_s1];
+    if ((unsigned)blk >= (unsigned)p.num_blocks) blk = 0;   // recorded by score_kernel
+    float f[8];
+    to_f32x8(T{}, *reinterpret_cast<const uint4*>(bounds + (int64_t)blk * p.b_s0), f);
+    double x = 0.0;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) x = fma((double)f[c], sh.side[e * 8 + c], x);
+#pragma unroll
+    for (int o = LP / 2; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    return order_key(x);
+  };
+  // Lists the pages with near_lo <= key <= near_hi (the first kNear) and counts those above.
+  const auto list_near = [&](uint32_t near_lo, uint32_t near_hi) {
+    for (int i0 = warp * 32; i0 < N; i0 += kThr) {
+      const uint32_t k = i0 + lane < N ? keys[i0 + lane] : 0;
+      const int up = __popc(__ballot_sync(~0u, i0 + lane < N && k > near_hi));
+      if (lane == 0 && up) atomicAdd(&sh.above, up);
+      if (i0 + lane < N && k >= near_lo && k <= near_hi) {
+        const int c = atomicAdd(&sh.near, 1);
+        if (c < kNear) sh.near_page[c] = i0 + lane;
+      }
+    }
+    __syncthreads();
+  };
+  // How many of the listed pages come before listed page `tid`.
+  const auto better = [&](int near, uint64_t mine) {
+    const int page = sh.near_page[tid];
+    int n = 0;
+    for (int c = 0; c < near; ++c)
+      n += sh.near_key[c] > mine || (sh.near_key[c] == mine && sh.near_page[c] < page);
+    return n;
+  };
+  // The open ones of the listed pages by 64-bit scores; their keys become the largest, those
+  // of the others the smallest (the scratch or its copy: this CTA's own).
+  const auto settle = [&](int near, int open) {
+    for (int c = warp; c < near; c += kThr / 32) {
+      const uint64_t k = score(sh.near_page[c]);
+      if (lane == 0) sh.near_key[c] = k;
+    }
+    __syncthreads();
+    if (tid < near) keys[sh.near_page[tid]] = better(near, sh.near_key[tid]) < open ? ~0u : 0;
+    __syncthreads();
+  };
+
+  // ---- ordinary scores: one histogram of 2048 equal parts of the keys' range, then the few
+  // pages of the border's part, and those within reach of it, one by one ----
+  if (N <= kPickCache && k_hi < ~0u && reach < INFINITY) {
+    uint32_t* bins = reinterpret_cast<uint32_t*>(sh.bins);
+    const int s = max(0, 21 - __clz(k_hi - k_lo));   // (k_hi - k_lo) >> s < 2048
+    for (int i = tid; i < N; i += kThr) atomicAdd(&bins[(keys[i] - k_lo) >> s], 1u);
+    __syncthreads();
+    // from the highest bin down, eight bins to each of 256 threads
+    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+    if (warp < 8) {
+      x = sh.bins[kBins / 4 - 1 - 2 * tid];
+      y = sh.bins[kBins / 4 - 2 - 2 * tid];
+    }
+    const uint32_t mine = x.x + x.y + x.z + x.w + y.x + y.y + y.z + y.w;
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31 && warp < 8) sh.scan[warp] = incl;
+    __syncthreads();
+    for (int w = 0; w < min(warp, 8); ++w) incl += sh.scan[w];
+    if (warp < 8 && incl >= (uint32_t)need && incl - mine < (uint32_t)need) {
+      const uint32_t c[8] = {x.w, x.z, x.y, x.x, y.w, y.z, y.y, y.x};
+      uint32_t sum = incl - mine;
+      int j = 0;
+#pragma unroll
+      for (int u = 0; u < 7; ++u) {
+        sum += c[u];
+        j += sum < (uint32_t)need;
+      }
+      sh.found[0] = kBins - 1 - 8 * tid - j;
+    }
+    __syncthreads();
+    const uint32_t first = k_lo + (sh.found[0] << s), last = first + ((1u << s) - 1);
+    const uint32_t near_lo = max(order_key(key_value(first) - reach), 1u) - 1;
+    const uint32_t near_hi = min(order_key(key_value(min(last, k_hi)) + reach), ~0u - 2) + 1;
+    list_near(near_lo, near_hi);
+    const int near = sh.near, open = need - sh.above;
+    if (near <= kNear) {
+      bool chosen = false;
+      if (tid < near) sh.near_key[tid] = keys[sh.near_page[tid]];
+      __syncthreads();
+      if (tid < near) {
+        chosen = better(near, sh.near_key[tid]) < open;
+        if (chosen) atomicMin(&sh.in, (uint32_t)sh.near_key[tid]);
+        else atomicMax(&sh.off, (uint32_t)sh.near_key[tid]);
+      }
+      __syncthreads();
+      if (near == open || err == 0.f || key_value(sh.in) - key_value(sh.off) > reach) {
+        if (tid < near) keys[sh.near_page[tid]] = chosen ? ~0u : 0;
+        __syncthreads();
+      } else {
+        settle(near, open);
+      }
+      write_selected<kThr>(N, sh, [&](int i) { return keys[i] > near_hi ? 1 : 0; }, 0, out, p.sinks);
+      return;
+    }
+    __syncthreads();
+    if (tid == 0) sh.above = sh.near = 0;
+    __syncthreads();
+  }
+
+  // ---- long units, many equal scores, infinities: the border by radix selection; the keys
+  // >= border are selected, all of them or, lowest index first, `rest` of the equal ones ----
+  int shift, rest = need, level;
+  uint32_t border;
+  find_border<kThr>(keys, N, k_lo, k_hi, sh, shift, border, rest, level);
+  const bool whole = level == rest;
+  border = shift < 32 ? border << shift : 0;
+  // the scores next to the border on both sides
+  uint32_t in = ~0u, off = 0;
+  for (int i = tid; i < N; i += kThr) {
+    const uint32_t k = keys[i];
+    if (k >= border) in = min(in, k);
+    else off = max(off, k);
+  }
+  in = __reduce_min_sync(~0u, in);
+  off = __reduce_max_sync(~0u, off);
+  if (lane == 0) {
+    sh.lo[warp] = in;
+    sh.hi[warp] = off;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThr / 32; ++w) {
+    in = min(in, (uint32_t)sh.lo[w]);
+    off = max(off, (uint32_t)sh.hi[w]);
+  }
+  const bool nan = in == ~0u;                        // the border lies among NaN scores: all the same
+  const float at = key_value(in);
+  // sure: every selected score is further above every other than the error can move them
+  if (err == 0.f || nan || (whole && at - key_value(off) > reach)) {
+    write_selected<kThr>(N, sh, [&](int i) {
+      const uint32_t k = keys[i];
+      return k > border || (whole && k == border) ? 1 : k == border ? 2 : 0;
+    }, rest, out, p.sinks);
+    return;
+  }
+
+  // 64-bit scores of the pages within reach of the border; above it all are selected,
+  // below it none. Not a number of an error: every page but the NaN ones.
+  uint32_t near_lo = 0, near_hi = ~0u - 1;
+  if (reach < INFINITY) {
+    near_lo = max(order_key(at - reach), 1u) - 1;
+    near_hi = min(order_key(at + reach), ~0u - 2) + 1;
+  }
+  list_near(near_lo, near_hi);
+  const int near = sh.near, open = need - sh.above;  // pages to be told apart, and how many of them are selected
+  if (near <= kNear) {
+    settle(near, open);
+    write_selected<kThr>(N, sh, [&](int i) { return keys[i] > near_hi ? 1 : 0; }, 0, out, p.sinks);
+    return;
+  }
+  // many of them (equal pages, or no usable error): all keys in 64 bits
+  uint64_t* exact = p.exact + (int64_t)unit * p.key_stride;
+  uint64_t lo64 = ~0ull, hi64 = 0;
+  for (int i0 = warp * 32; i0 < N; i0 += kThr) {
+    const uint32_t k = i0 + lane < N ? keys[i0 + lane] : 0;
+    uint64_t x = k > near_hi ? ~0ull : 0;
+    for (uint32_t m = __ballot_sync(~0u, i0 + lane < N && k >= near_lo && k <= near_hi); m; m &= m - 1) {
+      const uint64_t y = score(i0 + __ffs(m) - 1);
+      if (lane == __ffs(m) - 1) x = y;
+    }
+    if (i0 + lane < N) {
+      exact[i0 + lane] = x;
+      lo64 = min(lo64, x);
+      hi64 = max(hi64, x);
     }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    k_lo = min(k_lo, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)k_lo, o));
-    k_hi = max(k_hi, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)k_hi, o));
+    lo64 = min(lo64, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)lo64, o));
+    hi64 = max(hi64, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)hi64, o));
   }
   if (lane == 0) {
-    warp_lo[warp] = k_lo;
-    warp_hi[warp] = k_hi;
+    sh.lo[warp] = lo64;
+    sh.hi[warp] = hi64;
   }
-  if (tid < 256) hist[tid] = 0;
-  __syncthreads();
+  __syncthreads();                                   // also orders this CTA's writes of `exact` before its reads
 #pragma unroll
-  for (int w = 0; w < kPickWarps; ++w) {
-    k_lo = min(k_lo, warp_lo[w]);
-    k_hi = max(k_hi, warp_hi[w]);
+  for (int v = 0; v < kThr / 32; ++v) {
+    lo64 = min(lo64, sh.lo[v]);
+    hi64 = max(hi64, sh.hi[v]);
   }
-
-  // ---- the border: key >> shift == border for the last selected ones, `rest` of them ----
-  const int top_bit = k_lo == k_hi ? -1 : 63 - __clzll((long long)(k_lo ^ k_hi));
-  int shift = top_bit + 1;                           // bits above are the same in all keys
-  uint64_t border = shift >= 64 ? 0 : k_lo >> shift;
-  int rest = p.top - p.sinks - p.recent;             // < N
-  while (shift > 0) {
-    const int bits = min(8, shift), ns = shift - bits;
-    for (int i = tid; i < N; i += kAhead * kPickThreads) {
-      uint64_t k[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) k[u] = keys[min(i + u * kPickThreads, N - 1)];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (i + u * kPickThreads < N && (shift >= 64 || (k[u] >> shift) == border))
-          atomicAdd(&hist[(uint32_t)(k[u] >> ns) & ((1u << bits) - 1)], 1u);
-    }
-    __syncthreads();
-    // bins from the highest down: thread t < 256 has bin 255 - t
-    uint32_t mine = 0, incl = 0;
-    if (warp < 8) {
-      mine = incl = hist[255 - tid];
-      hist[255 - tid] = 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(~0u, incl, o);
-        if (lane >= o) incl += v;
-      }
-      if (lane == 31) scan[warp] = incl;
-    }
-    __syncthreads();
-    if (warp < 8) {
-      for (int w = 0; w < warp; ++w) incl += scan[w];
-      if (incl >= (uint32_t)rest && incl - mine < (uint32_t)rest) {
-        found[0] = 255 - (uint32_t)tid;
-        found[1] = (uint32_t)rest - (incl - mine);
-        found[2] = mine;
-      }
-    }
-    __syncthreads();
-    border = (border << bits) | found[0];
-    rest = (int)found[1];
-    shift = ns;
-    if (found[2] == found[1]) break;                 // the whole bin is selected
-  }
-
-  // ---- the selected pages in ascending order: a warp per consecutive part ----
-  const int per = ((N + kPickWarps - 1) / kPickWarps + 31) & ~31;
-  const int w0 = min(warp * per, N), w1 = min(w0 + per, N);
-  int gt = 0, eq = 0;
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const bool in = i0 + lane < w1;
-    const uint64_t k = in ? keys[i0 + lane] >> shift : 0;
-    gt += __popc(__ballot_sync(~0u, in && k > border));
-    eq += __popc(__ballot_sync(~0u, in && k == border));
-  }
-  if (lane == 0) {
-    n_gt[warp] = gt;
-    n_eq[warp] = eq;
-  }
-  __syncthreads();
-  gt = eq = 0;
-  for (int w = 0; w < warp; ++w) {
-    gt += n_gt[w];
-    eq += n_eq[w];
-  }
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const bool in = i0 + lane < w1;
-    const uint64_t k = in ? keys[i0 + lane] >> shift : 0;
-    const uint32_t mg = __ballot_sync(~0u, in && k > border), me = __ballot_sync(~0u, in && k == border);
-    const uint32_t below = (1u << lane) - 1u;
-    const int gb = gt + __popc(mg & below), eb = eq + __popc(me & below);
-    if (in && (k > border || (k == border && eb < rest))) out[p.sinks + gb + min(eb, rest)] = p.sinks + i0 + lane;
-    gt += __popc(mg);
-    eq += __popc(me);
-  }
+  uint64_t border64;
+  rest = need;
+  find_border<kThr>(exact, N, lo64, hi64, sh, shift, border64, rest, level);
+  write_selected<kThr>(N, sh, [&](int i) {
+    const uint64_t k = exact[i] >> shift;
+    return k > border64 ? 1 : k == border64 ? 2 : 0;
+  }, rest, out, p.sinks);
 }
 
 template <typename T, int D>
 int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
   const int64_t units = (int64_t)p.n * p.num_kv_heads;
-  if (units * ((p.key_stride + kRun - 1) / kRun) > 0x7fffffff) return STARKV_EINVAL;   // 32-bit run numbers
+  p.run_stride = (p.key_stride + kRun - 1) / kRun;
+  if (units * p.run_stride > 0x7fffffff) return STARKV_EINVAL;   // 32-bit run numbers
+  p.runs = reinterpret_cast<uint4*>(p.scratch);
+  p.exact = reinterpret_cast<uint64_t*>(p.runs + units * p.run_stride);
+  p.keys = reinterpret_cast<uint32_t*>(p.exact + units * p.key_stride);
   const void* fn = (const void*)score_kernel<T, D>;
   if (const int st = allow_smem(fn, kRingBytes)) return st;
   void* args[] = {&p};
   if (p.key_stride > p.top) {   // else no sequence has pages to choose from
-    const int64_t runs = units * ((p.key_stride + kRun - 1) / kRun);
-    const int64_t grid = std::min<int64_t>(3 * num_sms, runs);
+    const int64_t grid = std::min<int64_t>(3 * num_sms, units * p.run_stride);
     if (cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), args, kRingBytes, stream) != cudaSuccess)
       return STARKV_ECUDA;
   }
@@ -393,11 +757,13 @@ int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)units);
-  cfg.blockDim = dim3(kPickThreads);
+  const bool few = units <= num_sms && p.key_stride > 1024;   // 281 pages: 11.0 against 12.1 us with 1024 threads
+  cfg.blockDim = dim3(few ? 1024 : 256);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = p.key_stride > p.top;   // behind score_kernel alone may the launch come early
-  return cudaLaunchKernelExC(&cfg, (const void*)pick_kernel, args) == cudaSuccess ? STARKV_OK : STARKV_ECUDA;
+  const void* pick = few ? (const void*)pick_kernel<T, D, 1024> : (const void*)pick_kernel<T, D, 256>;
+  return cudaLaunchKernelExC(&cfg, pick, args) == cudaSuccess ? STARKV_OK : STARKV_ECUDA;
 }
 
 template <typename T, int D>
@@ -413,6 +779,10 @@ int launch_bounds_typed(PageBoundsParams p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+size_t select_scratch_bytes(int64_t units, int64_t pages) {
+  return (size_t)units * (pages * 12 + (pages + kRun - 1) / kRun * 16);
+}
 
 int launch_page_bounds(const PageBoundsParams& p, int dtype, int head_dim, cudaStream_t stream) {
   if (dtype == STARKV_BF16)

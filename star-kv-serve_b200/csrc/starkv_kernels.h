@@ -174,7 +174,11 @@ struct SelectPagesParams {
   int max_blocks, num_blocks, block_size;
   const int32_t* seq_lens;
   int max_len, n, num_kv_heads, group, top, sinks, recent;
-  uint64_t* keys; int64_t key_stride;                // scratch [n, KV heads, pages of the longest sequence]
+  void* scratch; int64_t key_stride;                 // pages of the longest sequence
+  // set by the launch, in `scratch`: per run of pages {error, smallest key, largest key};
+  // order keys of the 32-bit scores and, where they do not decide, of the 64-bit ones
+  uint4* runs; int64_t run_stride;                   // [n, KV heads, run_stride]
+  uint32_t* keys; uint64_t* exact;                   // [n, KV heads, key_stride]
   int32_t* pages; int64_t pg_s0, pg_s1;              // [n, KV heads, top]
   int32_t* status;
 };
@@ -227,6 +231,7 @@ int allow_smem(const void* fn, int bytes);
 size_t paged_attn_workspace_bytes(int rows, int head_dim, int max_tokens);
 int launch_paged_attn(const PagedAttnParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
 int launch_page_bounds(const PageBoundsParams& p, int dtype, int head_dim, cudaStream_t stream);
+size_t select_scratch_bytes(int64_t units, int64_t pages);
 int launch_select_pages(SelectPagesParams p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
 int launch_norm_rope(const NormRopeParams& p, int dtype, int head_dim, int num_sms, cudaStream_t stream);
 int launch_prefill(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const PrefillParams& p,

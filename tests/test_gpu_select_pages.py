@@ -91,6 +91,53 @@ def test_ties_go_to_the_lowest_page():
     run([16 * 700] * 40, 4, 4, top=10, levels=1, D=64, seed=5)
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_scores_that_32_bits_cannot_tell_apart(dtype, D):
+    """A common part of 256 (its last place in f32: 2^-15) and differences of multiples of
+    2^-20: the order is only there in 64 bits. Some pages stand clearly above and below."""
+    from starkv_b200.kernels.paged_attention import select_pages
+    dev = cuda()
+    g = torch.Generator(device=dev).manual_seed(11)
+    n, P, Hkv = 3, 900, 2
+    bt = table(n, P, 1)
+    b = torch.zeros(n * P + 1, Hkv, D, device=dev)
+    b[..., 0] = 16
+    j = torch.randint(0, 200, b.shape[:2], generator=g, device=dev)
+    b[..., 1] = j * 2.0 ** -16                            # bf16 and f16 hold them
+    far = torch.rand(b.shape[:2], generator=g, device=dev)
+    b[..., 2] = torch.where(far < 0.01, 1.0, torch.where(far > 0.9, -1.0, 0.0))
+    bounds = torch.stack([b, b], 2).to(dtype)
+    assert torch.equal(bounds[:, :, 0].float(), b)
+    q = torch.zeros(n, 4, D, device=dev)
+    q[:, ::2, 0], q[:, ::2, 1], q[:, ::2, 2] = 16, 2.0 ** -4, 1
+    q = q.to(dtype)
+    sl = torch.tensor([16 * P, 16 * 70, 16 * 400], dtype=torch.int32, device=dev)
+    for top in (40, 65):
+        got = select_pages(q, bounds, bt, sl, 16 * P, 16, top)
+        assert torch.equal(got.cpu(), expected(q, bounds, bt, sl.tolist(), 16, top, 1, 1))
+
+
+def test_infinite_bounds():
+    from starkv_b200.kernels.paged_attention import select_pages
+    dev = cuda()
+    bounds = torch.randn(301, 1, 2, 128, device=dev).sort(2).values.to(torch.bfloat16)
+    bounds[50, 0, 1, 3] = bounds[200, 0, 1, 3] = float("inf")
+    bounds[90, 0, 0, 3] = bounds[91, 0, 1, 4] = float("-inf")
+    bt = torch.arange(1, 301, device=dev, dtype=torch.int32)[None]
+    q = torch.randn(1, 2, 128, device=dev).abs().to(torch.bfloat16)
+    q[:, 0, 7] = -1
+    sl = torch.tensor([4800], dtype=torch.int32, device=dev)
+    for top in (1, 2, 30, 298, 299):
+        got = select_pages(q, bounds, bt, sl, 4800, 16, top, sinks=0, recent=0)
+        up, down = q.double().clamp(min=0).sum(1), q.double().clamp(max=0).sum(1)
+        B = bounds[1:, 0].double()
+        s = (up * B[:, 1] + down * B[:, 0]).sum(-1)       # 0 times an infinity: NaN, which ranks first
+        s = torch.where(s.isnan(), float("inf"), s) + torch.where(s.isnan(), 1.0, 0.0)
+        nan = (up * B[:, 1] + down * B[:, 0]).sum(-1).isnan()
+        order = sorted(range(300), key=lambda i: (not bool(nan[i]), -float(s[i]), i))[:top]
+        assert got[0, 0].tolist() == sorted(order), top
+
+
 def test_nan_bounds_rank_first():
     from starkv_b200.kernels.paged_attention import select_pages
     dev = cuda()
