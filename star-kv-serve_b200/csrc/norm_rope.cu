@@ -17,8 +17,8 @@ namespace starkv {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kManyRows = 256;   // rows per SM from which a group takes 8 rows and not 2
+constexpr int kThreads = 128;
+constexpr int kManyRows = 256;   // rows per SM from which a warp takes 4 steps and not one
 
 __device__ __forceinline__ float4 load4(const void* p, int64_t i, int dtype) {
   if (dtype == STARKV_F32) return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
@@ -63,38 +63,92 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
-// A group of D / 8 lanes takes up to kPer consecutive heads of the queries, keys or values
-// of one token: the position's table values and the weight are loaded once for them, and
-// kPer rows are in flight.
-template <typename T, int D, int kPer>
-__global__ void __launch_bounds__(kThreads, 3) norm_rope_kernel(const NormRopeParams p, unsigned q_chunks,
-                                                                unsigned k_chunks, unsigned chunks, unsigned items) {
-  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes;
-  const int j = threadIdx.x % kLanes;
-  const unsigned item = blockIdx.x * kGroups + threadIdx.x / kLanes;
-  const bool live = item < items;                      // groups share a warp: all take part in the shuffles
-  const unsigned t = live ? item / chunks : 0, chunk = live ? item - t * chunks : 0;
+// A warp takes up to kSteps * G heads of the queries, keys or values of one token, G = 32 *
+// 8 / D heads a step: token, kind, table row and cache slot are the warp's, so a row costs
+// little more than its own arithmetic (8191 tokens of 48 heads, f16: 41 us, 5.0 TB/s; with
+// token and heads chosen per group of lanes 193 instructions a warp and step, and 51 us).
+template <typename T, int D, int kSteps>
+__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeParams p, unsigned q_chunks,
+                                                             unsigned k_chunks, unsigned chunks, unsigned items) {
+  constexpr int kLanes = D / 8, G = 32 / kLanes;
+  constexpr int kAhead = kSteps < 4 ? kSteps : 4;      // steps in flight
+  const int lane = threadIdx.x & 31;
+  const unsigned item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (item >= items) return;
+  const unsigned t = item / chunks, chunk = item - t * chunks;
   const int kind = chunk < q_chunks ? 0 : chunk < q_chunks + k_chunks ? 1 : 2;   // query, key, value
-  const int h0 = kPer * (int)(chunk - (kind == 0 ? 0 : kind == 1 ? q_chunks : q_chunks + k_chunks));
-  const int count = live ? min(kPer, (kind == 0 ? p.num_heads : p.num_kv_heads) - h0) : 0;
-  const int64_t step = kind == 0 ? p.q_s1 : kind == 1 ? p.k_s1 : p.v_s1;
+  const int j = lane % kLanes, g = lane / kLanes;
+  const int h0 = kSteps * G * (int)(chunk - (kind == 0 ? 0 : kind == 1 ? q_chunks : q_chunks + k_chunks)) + g;
+  const int heads = (kind == 0 ? p.num_heads : p.num_kv_heads) - h0 + G - 1;
+  const int count = heads / G, most = (heads + g) / G;   // heads of this group (also <= 0), of group 0
   // this lane's channels: lo .. lo + 3 and hi .. hi + 3; behind the rotated width eight in a row
   const int pairs = p.rot / 8;
-  const bool turns = j < pairs && kind < 2;
   const int lo = j < pairs ? 4 * j : p.rot + 8 * (j - pairs), hi = j < pairs ? lo + p.rot / 2 : lo + 4;
-  const T* src = reinterpret_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) +
-                 t * (kind == 0 ? p.q_s0 : kind == 1 ? p.k_s0 : p.v_s0) + h0 * step;
-  uint2 raw_lo[kPer], raw_hi[kPer];
+  const int64_t s0 = kind == 0 ? p.q_s0 : kind == 1 ? p.k_s0 : p.v_s0;
+  const int64_t s1 = kind == 0 ? p.q_s1 : kind == 1 ? p.k_s1 : p.v_s1;
+  const T* src = reinterpret_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + t * s0 + h0 * s1 + lo;
+  const int64_t step = G * s1;
+  uint2 raw[kAhead][2];
+  const auto load = [&](int s) {                       // steps s .. s + kAhead - 1
 #pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    raw_lo[u] = u < count ? *reinterpret_cast<const uint2*>(src + u * step + lo) : make_uint2(0, 0);
-    raw_hi[u] = u < count ? *reinterpret_cast<const uint2*>(src + u * step + hi) : make_uint2(0, 0);
+    for (int u = 0; u < kAhead; ++u) {
+      raw[u][0] = raw[u][1] = make_uint2(0, 0);
+      if (s + u < count) {
+        raw[u][0] = *reinterpret_cast<const uint2*>(src);
+        raw[u][1] = *reinterpret_cast<const uint2*>(src + (hi - lo));
+      }
+      src += step;
+    }
+  };
+  load(0);
+
+  // where the rows go: queries to q_out, keys and values to the cache, keys to k_out as well
+  T *to = nullptr, *also = nullptr;
+  int64_t to_step = 0, also_step = 0;
+  if (kind == 0) {
+    to = reinterpret_cast<T*>(p.q_out) + t * p.qo_s0 + h0 * p.qo_s1 + lo;
+    to_step = G * p.qo_s1;
+  } else {
+    if (p.k_cache) {
+      const int64_t slot = load_slot(p.slots, t, p.slot_dtype);
+      if (slot >= (int64_t)p.num_blocks * p.block_size) {
+        record_status(p.status, STARKV_EBOUNDS);
+      } else if (slot >= 0) {                          // negative: padding, not written
+        // a 64-bit division is some hundred instructions
+        const int64_t blk = slot <= 0x7fffffff ? (unsigned)slot / (unsigned)p.block_size : slot / p.block_size;
+        const int64_t off = slot - blk * p.block_size;
+        const int64_t c2 = kind == 1 ? p.kc_s2 : p.vc_s2;
+        to = reinterpret_cast<T*>(kind == 1 ? p.k_cache : p.v_cache) + blk * (kind == 1 ? p.kc_s0 : p.vc_s0) +
+             off * (kind == 1 ? p.kc_s1 : p.vc_s1) + h0 * c2 + lo;
+        to_step = G * c2;
+      }
+    }
+    if (kind == 1 && p.k_out) {
+      also = reinterpret_cast<T*>(p.k_out) + t * p.ko_s0 + h0 * p.ko_s1 + lo;
+      also_step = G * p.ko_s1;
+    }
   }
+  if (kind == 2) {
+    if (!to) return;
+#pragma unroll
+    for (int s = 0; s < kSteps; s += kAhead) {
+      if (s) load(s);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s + u < count) {
+          *reinterpret_cast<uint2*>(to) = raw[u][0];
+          *reinterpret_cast<uint2*>(to + (hi - lo)) = raw[u][1];
+        }
+        to += to_step;
+      }
+    }
+    return;
+  }
+  const bool has_to = to != nullptr, has_also = also != nullptr;
 
   // out_lo = inv * (x_lo a + x_hi b), out_hi = inv * (x_hi c + x_lo d): the weight is in a .. d already
   float4 a = make_float4(1.f, 1.f, 1.f, 1.f), b = make_float4(0.f, 0.f, 0.f, 0.f), c = a, d = b;
-  const void* w = kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr;
-  if (turns && live) {
+  if (j < pairs) {
     int64_t pos = load_slot(p.positions, t, p.pos_dtype);
     if (pos < 0 || pos >= p.table_rows) {
       record_status(p.status, STARKV_EBOUNDS);
@@ -105,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, 3) norm_rope_kernel(const NormRopePa
     d = load4(p.table, at + p.rot / 2, p.table_dtype);
     b = make_float4(-d.x, -d.y, -d.z, -d.w);
   }
+  const void* w = kind == 0 ? p.q_weight : p.k_weight;
   if (w) {
     const float4 gl = load4(w, lo, p.w_dtype), gh = load4(w, hi, p.w_dtype);
     a = make_float4(a.x * gl.x, a.y * gl.y, a.z * gl.z, a.w * gl.w);
@@ -112,73 +167,70 @@ __global__ void __launch_bounds__(kThreads, 3) norm_rope_kernel(const NormRopePa
     c = make_float4(c.x * gh.x, c.y * gh.y, c.z * gh.z, c.w * gh.w);
     d = make_float4(d.x * gl.x, d.y * gl.y, d.z * gl.z, d.w * gl.w);
   }
-  // where the rows go: q_out, or k_out and the cache
-  T* out = kind == 0   ? reinterpret_cast<T*>(p.q_out) + t * p.qo_s0 + h0 * p.qo_s1
-           : kind == 1 ? reinterpret_cast<T*>(p.k_out) + t * p.ko_s0 + h0 * p.ko_s1
-                       : nullptr;
-  if (kind == 1 && !p.k_out) out = nullptr;
-  const int64_t out_step = kind == 0 ? p.qo_s1 : p.ko_s1;
-  T* cache = nullptr;
-  const int64_t cache_step = kind == 1 ? p.kc_s2 : p.vc_s2;
-  if (p.k_cache && kind > 0 && live) {
-    const int64_t slot = load_slot(p.slots, t, p.slot_dtype);
-    if (slot >= (int64_t)p.num_blocks * p.block_size) {
-      record_status(p.status, STARKV_EBOUNDS);
-    } else if (slot >= 0) {                            // negative: padding, not written
-      // a 64-bit division is some hundred instructions
-      const int64_t blk = slot <= 0x7fffffff ? (unsigned)slot / (unsigned)p.block_size : slot / p.block_size;
-      const int64_t off = slot - blk * p.block_size;
-      cache = kind == 1 ? reinterpret_cast<T*>(p.k_cache) + blk * p.kc_s0 + off * p.kc_s1 + h0 * p.kc_s2
-                        : reinterpret_cast<T*>(p.v_cache) + blk * p.vc_s0 + off * p.vc_s1 + h0 * p.vc_s2;
-    }
-  }
-  const bool norms = p.q_weight || p.k_weight;
+  const float2 a0 = make_float2(a.x, a.y), a1 = make_float2(a.z, a.w), b0 = make_float2(b.x, b.y),
+               b1 = make_float2(b.z, b.w), c0 = make_float2(c.x, c.y), c1 = make_float2(c.z, c.w),
+               d0 = make_float2(d.x, d.y), d1 = make_float2(d.z, d.w);
 #pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    uint2 res_lo = raw_lo[u], res_hi = raw_hi[u];
-    const float2 l0 = unpack(T{}, res_lo.x), l1 = unpack(T{}, res_lo.y);
-    const float2 h0 = unpack(T{}, res_hi.x), h1 = unpack(T{}, res_hi.y);
-    float inv = 1.f;
-    if (norms) {
-      const float2 q = fma2(h1, h1, fma2(h0, h0, fma2(l1, l1, mul2(l0, l0))));
-      float ss = q.x + q.y;
+  for (int s = 0; s < kSteps; s += kAhead) {
+    if (s) {
+      if (s >= most) break;
+      load(s);
+    }
+    float inv[kAhead];
+    if (w) {
 #pragma unroll
-      for (int o = kLanes / 2; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-      if (w) inv = rsqrtf(ss * (1.f / D) + p.eps);     // within 2^-22
+      for (int u = 0; u < kAhead; ++u) {
+        const float2 l0 = unpack(T{}, raw[u][0].x), l1 = unpack(T{}, raw[u][0].y);
+        const float2 h0v = unpack(T{}, raw[u][1].x), h1v = unpack(T{}, raw[u][1].y);
+        const float2 q = fma2(h1v, h1v, fma2(h0v, h0v, fma2(l1, l1, mul2(l0, l0))));
+        inv[u] = q.x + q.y;
+      }
+#pragma unroll
+      for (int o = kLanes / 2; o; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) inv[u] += __shfl_xor_sync(~0u, inv[u], o);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) inv[u] = rsqrtf(inv[u] * (1.f / D) + p.eps);   // within 2^-22
     }
-    if (u >= count) continue;
-    if (kind < 2) {
-      const float2 iv = make_float2(inv, inv);
-      const float2 a0 = make_float2(a.x, a.y), a1 = make_float2(a.z, a.w), b0 = make_float2(b.x, b.y),
-                   b1 = make_float2(b.z, b.w), c0 = make_float2(c.x, c.y), c1 = make_float2(c.z, c.w),
-                   d0 = make_float2(d.x, d.y), d1 = make_float2(d.z, d.w);
-      res_lo.x = round2(T{}, mul2(iv, fma2(h0, b0, mul2(l0, a0))));
-      res_lo.y = round2(T{}, mul2(iv, fma2(h1, b1, mul2(l1, a1))));
-      res_hi.x = round2(T{}, mul2(iv, fma2(l0, d0, mul2(h0, c0))));
-      res_hi.y = round2(T{}, mul2(iv, fma2(l1, d1, mul2(h1, c1))));
-    }
-    if (out) {
-      *reinterpret_cast<uint2*>(out + u * out_step + lo) = res_lo;
-      *reinterpret_cast<uint2*>(out + u * out_step + hi) = res_hi;
-    }
-    if (cache) {
-      *reinterpret_cast<uint2*>(cache + u * cache_step + lo) = res_lo;
-      *reinterpret_cast<uint2*>(cache + u * cache_step + hi) = res_hi;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float2 l0 = unpack(T{}, raw[u][0].x), l1 = unpack(T{}, raw[u][0].y);
+      const float2 h0v = unpack(T{}, raw[u][1].x), h1v = unpack(T{}, raw[u][1].y);
+      float2 x0 = fma2(h0v, b0, mul2(l0, a0)), x1 = fma2(h1v, b1, mul2(l1, a1));
+      float2 y0 = fma2(l0, d0, mul2(h0v, c0)), y1 = fma2(l1, d1, mul2(h1v, c1));
+      if (w) {
+        const float2 iv = make_float2(inv[u], inv[u]);
+        x0 = mul2(iv, x0);
+        x1 = mul2(iv, x1);
+        y0 = mul2(iv, y0);
+        y1 = mul2(iv, y1);
+      }
+      const uint2 x = make_uint2(round2(T{}, x0), round2(T{}, x1)), y = make_uint2(round2(T{}, y0), round2(T{}, y1));
+      if (s + u < count) {
+        if (has_to) {
+          *reinterpret_cast<uint2*>(to) = x;
+          *reinterpret_cast<uint2*>(to + (hi - lo)) = y;
+        }
+        if (has_also) {
+          *reinterpret_cast<uint2*>(also) = x;
+          *reinterpret_cast<uint2*>(also + (hi - lo)) = y;
+        }
+      }
+      to += to_step;
+      also += also_step;
     }
   }
 }
 
-template <typename T, int D, int kPer>
-int launch_per(NormRopeParams p, cudaStream_t stream) {
-  constexpr int kGroups = kThreads / (D / 8);
-  unsigned qc = (p.num_heads + kPer - 1) / kPer;
-  unsigned kc = (p.num_kv_heads + kPer - 1) / kPer;
+template <typename T, int D, int kSteps>
+int launch_steps(const NormRopeParams& p, cudaStream_t stream) {
+  constexpr int heads = kSteps * (256 / D);            // of a warp
+  unsigned qc = (p.num_heads + heads - 1) / heads, kc = (p.num_kv_heads + heads - 1) / heads;
   unsigned chunks = qc + kc * (p.v ? 2 : 1);
-  const int64_t all = (int64_t)p.n * chunks;
-  if (all > 0x7fffffff) return STARKV_EINVAL;
-  unsigned items = (unsigned)all;
-  void* args[] = {&p, &qc, &kc, &chunks, &items};
-  return cudaLaunchKernel((const void*)norm_rope_kernel<T, D, kPer>, dim3((items + kGroups - 1) / kGroups),
+  if ((int64_t)p.n * chunks > 0x7fffffff) return STARKV_EINVAL;
+  unsigned items = (unsigned)p.n * chunks;
+  void* args[] = {const_cast<NormRopeParams*>(&p), &qc, &kc, &chunks, &items};
+  return cudaLaunchKernel((const void*)norm_rope_kernel<T, D, kSteps>, dim3((items + kThreads / 32 - 1) / (kThreads / 32)),
                           dim3(kThreads), args, 0, stream) == cudaSuccess
              ? STARKV_OK
              : STARKV_ECUDA;
@@ -187,7 +239,7 @@ int launch_per(NormRopeParams p, cudaStream_t stream) {
 template <typename T, int D>
 int launch_typed(const NormRopeParams& p, int num_sms, cudaStream_t stream) {
   const int64_t rows = (int64_t)p.n * (p.num_heads + p.num_kv_heads * (p.v ? 2 : 1));
-  return rows > (int64_t)num_sms * kManyRows ? launch_per<T, D, 8>(p, stream) : launch_per<T, D, 2>(p, stream);
+  return rows > (int64_t)num_sms * kManyRows ? launch_steps<T, D, 4>(p, stream) : launch_steps<T, D, 1>(p, stream);
 }
 
 }  // namespace
