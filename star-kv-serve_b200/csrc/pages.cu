@@ -191,21 +191,27 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
   const int d = (e * 8) % D;
   const bool upper = e * 8 >= D;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // pick_kernel waits for all of this one
-  const auto count = [&](int b) { return (competing(p, pages_of(p, b)) + kRun - 1) / kRun * p.num_kv_heads; };
+  // The warps of a CTA take the same pages of up to eight KV heads, whose bounds lie side by
+  // side: 4 KB of a page are read together where a warp alone reads 512 bytes.
+  const int abreast = min(p.num_kv_heads, kWarps), groups = (p.num_kv_heads + abreast - 1) / abreast;
+  const int parts = kWarps / abreast;                // shares of one CTA
+  if (warp >= parts * abreast) return;
+  const auto count = [&](int b) { return (competing(p, pages_of(p, b)) + kRun - 1) / kRun * groups; };
   FlatItems<decltype(count)> all(count, p.n, lane);
-  const int shares = min((int)gridDim.x * kWarps, all.total);
-  const int share = blockIdx.x + warp * gridDim.x;   // a warp of every CTA before the second of one
+  const int shares = min((int)gridDim.x * parts, all.total);
+  const int share = blockIdx.x + warp / abreast * gridDim.x;
   if (share >= shares) return;
   const int g1 = share_begin(all.total, share + 1, shares);
   int g = share_begin(all.total, share, shares);
   int b, first;
   all.place(g, b, first);
   int N = competing(p, pages_of(p, b)), runs = (N + kRun - 1) / kRun;
-  int hk = (g - first) / runs, run = (g - first) % runs;
+  int group = (g - first) / runs, run = (g - first) % runs;
 
   while (g < g1) {
     // the share's runs of this (sequence, KV head)
     const int here = min(runs - run, g1 - g);
+    const int hk = min(group * abreast + warp % abreast, p.num_kv_heads - 1);   // the last group: the last head again
     const int i0 = run * kRun, i1 = min(i0 + here * kRun, N);   // competing pages i0 .. i1 - 1
     const int steps = (i1 - i0 + kPer - 1) / kPer;
     const int32_t* bt = p.block_table + b * p.bt_s0 + (int64_t)p.sinks * p.bt_s1;
@@ -242,15 +248,18 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
     float size = 0.f;                                // sum of |w| of this lane's channels
 #pragma unroll
     for (int i = 0; i < 8; ++i) size += fabsf(w[i]);
-    issue(0);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (steps > 1) issue(1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < kRing - 1; ++j) {
+      if (j < steps) issue(j);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     uint32_t k_lo = ~0u, k_hi = 0;
     uint32_t largest = 0;                            // largest |bound| of this lane's channels, as a pair
     uint32_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride + i0;
     for (int j = 0; j < steps; ++j) {
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      if (j + kRing - 1 < steps) issue(j + kRing - 1);   // into the slots of step j - 1
+      asm volatile("cp.async.commit_group;" ::: "memory");
       float s[kStep];
 #pragma unroll
       for (int u = 0; u < kStep; ++u) {
@@ -263,8 +272,6 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
         s[u] = a.x + a.y;
         largest = max_abs2(T{}, max_abs2(T{}, max_abs2(T{}, largest, v.x), v.y), max_abs2(T{}, v.z, v.w));
       }
-      if (j + 2 < steps) issue(j + 2);   // into the slots of step j - 1
-      asm volatile("cp.async.commit_group;" ::: "memory");
       // sums over the LP lanes of a page: first steps that also halve the pages a lane holds
       int at = j * kPer + sub * kStep, o = LP / 2;
 #pragma unroll
@@ -306,8 +313,8 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     g += here;
     run = 0;
-    if (g < g1 && ++hk == p.num_kv_heads) {
-      hk = 0;
+    if (g < g1 && ++group == groups) {
+      group = 0;
       do N = ++b < p.n ? competing(p, pages_of(p, b)) : 0;
       while (N == 0 && b < p.n);
       if (b >= p.n) break;   // not reached: g < g1 <= total

@@ -16,9 +16,11 @@ There is no fallback: if the native library is missing the calls raise.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
-from .. import _lib, context_parallel
+from .. import _lib
 
 HEAD_DIMS = (64, 128)
 
@@ -123,7 +125,16 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
     m = l = None
     if return_partial:
         if d == 128:
-            out, m, l = context_parallel.partial_views(n, hq, query.device, partial)
+            nh = n * hq
+            if partial is None:
+                partial = query.new_empty(nh * 130, dtype=torch.float32)
+            elif partial.dtype is not torch.float32 or not partial.is_contiguous() or partial.numel() < nh * 130:
+                raise ValueError(f"{what}: partial must be a contiguous f32 buffer of at least {nh * 130} values")
+            # context_parallel.partial_views, by strides (three slices and views take 8 us)
+            at = partial.storage_offset()
+            out = partial.as_strided((n, hq, 128), (hq * 128, 128, 1), at)
+            m = partial.as_strided((n, hq), (hq, 1), at + nh * 128)
+            l = partial.as_strided((n, hq), (hq, 1), at + nh * 129)
         elif partial is not None:
             raise ValueError(f"{what}: the packed partial buffer holds head_dim 128")
         else:
@@ -157,12 +168,14 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
     return (out, m, l) if return_partial else out
 
 
+@lru_cache(maxsize=256)   # the calls' sizes repeat
 def workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int, max_tokens: int) -> int:
     """Scratch of one ``paged_attention_decode`` over at most ``max_tokens`` tokens per sequence."""
     return int(_lib.lib().starkv_paged_attention_workspace_bytes(num_heads, num_kv_heads, head_dim,
                                                                   min(int(max_tokens), 1 << 30)))
 
 
+@lru_cache(maxsize=256)
 def select_workspace_bytes(n: int, num_kv_heads: int, max_seq_len: int, block_size: int, top: int) -> int:
     """Scratch of one ``select_pages``; ``sparse_paged_decode`` takes this and ``workspace_bytes``
     of top * block_size tokens."""
