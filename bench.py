@@ -418,7 +418,7 @@ def model_measure(args, device, world, rank, dist_on, parallel, batch=None, cont
     if args.model_weights == "checkpoint":
         ckpt = synthetic_checkpoint_path(cfg, dist_on, rank)
     model = StarKVModel(cfg, device, quant=False, rank=rank if dist_on else 0, world=world if dist_on else 1,
-                        group=None, attn_parallel=split, checkpoint=ckpt)
+                        group=None, attn_parallel=split, checkpoint=ckpt, full_attention=args.full_attention)
     if ckpt is not None:
         if dist_on:
             dist.barrier()
@@ -1004,6 +1004,8 @@ def main():
                                                "heads, c4, model, bar, prefill")
     ap.add_argument("--model-weights", default="checkpoint", choices=["checkpoint", "random"],
                     help="config 5: K/V factors from a synthetic fused_weights.pt (default) or drawn in place")
+    ap.add_argument("--full-attention", default="stock", choices=["stock", "paged"],
+                    help="config 5's full-rank layers: vLLM's ops (default) or this library's paged operators")
     ap.add_argument("--batch", type=int, default=None, help="override the batch (profiling small cases)")
     ap.add_argument("--context", type=int, default=None, help="override the context (profiling small cases)")
     ap.add_argument("--no-bar", action="store_true", help="skip timing the reference's Triton kernels")

@@ -113,13 +113,18 @@ bool is_float_dtype(int d) { return d == STARKV_BF16 || d == STARKV_F16 || d == 
 int allow_smem(const void* fn, int bytes) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return STARKV_ECUDA;
-  static std::mutex guard;
-  static std::set<std::pair<const void*, int>> done;
-  std::lock_guard<std::mutex> lock(guard);
-  if (done.count({fn, dev})) return STARKV_OK;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return STARKV_ECUDA;
-  done.insert({fn, dev});
-  return STARKV_OK;
+  try {   // nothing may be thrown through the C entry points
+    static std::mutex guard;
+    static std::set<std::pair<const void*, int>> done;
+    std::lock_guard<std::mutex> lock(guard);
+    if (done.count({fn, dev})) return STARKV_OK;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      return STARKV_ECUDA;
+    done.insert({fn, dev});
+    return STARKV_OK;
+  } catch (...) {
+    return STARKV_ECUDA;
+  }
 }
 
 Workspace workspace_layout(int n, int num_heads, int num_kv_heads, int k_width, int v_rank, int max_seq_len) {

@@ -18,7 +18,9 @@ namespace starkv {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kManyRows = 256;   // rows per SM from which a warp takes 4 steps and not one
+// rows per SM from which a warp takes 4 steps and not one (48 rows a token: one token 3.0
+// against 3.4 us, 64 tokens the same, 256 tokens 4.2 against 3.5, 4096 tokens 37 against 22)
+constexpr int kManyRows = 24;
 
 __device__ __forceinline__ float4 load4(const void* p, int64_t i, int dtype) {
   if (dtype == STARKV_F32) return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);

@@ -92,7 +92,10 @@ def paged_attention_decode(
 
     ``pages`` (int32 [n, H_kv, top], as ``select_pages`` returns them): attend to the
     tokens of these pages of the sequence alone. A negative entry holds no token; each
-    listed page counts once per listing.
+    listed page counts once per listing; of a sequence with fewer than top pages only as
+    many entries are read as it has pages.
+
+    ``out`` may not overlap ``query``: a sequence is read by several CTAs.
 
     ``return_partial``: ``(out, m, l)`` for ``context_parallel.combine`` - out f32
     undivided, m / l f32 [n, H_q] the largest logit and the sum of exp(logit - m) - as
@@ -144,6 +147,8 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.shape != query.shape or out.dtype is not query.dtype or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must be [{n}, {hq}, {d}] in the cache's dtype, last dimension contiguous")
+    if out.data_ptr() == query.data_ptr() and n:
+        raise ValueError(f"{what}: out may not be the query itself")
     bounds = None if select is None else select[0]
     idx = _lib.same_device(what, query, k_cache, v_cache, block_table, seq_lens, pages, out, ws, status, bounds)
     if n == 0:

@@ -291,3 +291,58 @@ def test_a_page_listed_twice_counts_twice():
     out = paged_attention_decode(q, k, v, bt, sl, 64, 0.1, pages=two)
     ref, _, _, tol = reference(q, k, v, bt, sl, 0.1, pages=two)
     check(out, ref, tol)
+
+
+def test_cache_of_more_than_two_to_the_31_elements():
+    """Blocks at the far end of a cache whose offsets pass 32 bits, keys and values as views of
+    one tensor [blocks, 2, heads, block, 128]."""
+    from starkv_b200.kernels.paged_attention import empty_bounds, paged_attention_decode, sparse_paged_decode, \
+        update_page_bounds
+    from starkv_b200.kernels.qk_norm_rope import qk_norm_rope_write
+    dev = cuda()
+    if torch.cuda.mem_get_info(dev)[0] < 8 << 30:
+        pytest.skip("needs 8 GB")
+    Hkv, bs, n, T = 8, 16, 2, 300
+    blocks = (1 << 31) // (2 * Hkv * bs * 128) + 64
+    both = torch.empty(blocks, 2, Hkv, bs, 128, dtype=torch.bfloat16, device=dev)
+    k, v = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    assert (blocks - 1) * k.stride(0) > 1 << 31
+    per = -(-T // bs)
+    bt = (blocks - 1 - torch.arange(n * per, device=dev).view(n, per)).int()
+    qkv = torch.randn(n * T, 32 + 2 * Hkv, 128, device=dev).to(torch.bfloat16)
+    t = torch.arange(T, device=dev)
+    slots = (bt[:, t // bs].long() * bs + t % bs).reshape(-1)
+    cs = torch.cat([torch.ones(8, 64, device=dev), torch.zeros(8, 64, device=dev)], 1)     # no rotation
+    qk = qk_norm_rope_write(qkv[:, :32], qkv[:, 32:40], qkv[:, 40:], torch.zeros(n * T, dtype=torch.int64, device=dev), cs,
+                            k, v, slots)
+    assert torch.equal(qk, qkv[:, :32])
+    assert torch.equal(tokens_of(k, bt[1], t), qkv[T:, 32:40]) and torch.equal(tokens_of(v, bt[0], t), qkv[:T, 40:])
+    sl = torch.tensor([T, T - 9], dtype=torch.int32, device=dev)
+    q = qk[:2]
+    ref, _, _, tol = reference(q, k, v, bt, sl, 0.1)
+    check(paged_attention_decode(q, k, v, bt, sl, T, 0.1), ref, tol)
+    bounds = empty_bounds(k)
+    update_page_bounds(k, bounds, bt, sl, T, max_new=T)
+    out, pages = sparse_paged_decode(q, k, v, bounds, bt, sl, T, 0.1, 5)
+    ref, _, _, tol = reference(q, k, v, bt, sl, 0.1, pages=pages)
+    check(out, ref, tol)
+
+
+def test_shared_heads_of_an_expanded_cache():
+    """A cache whose head stride is 0 (one stored head seen as four)."""
+    from starkv_b200.kernels.paged_attention import paged_attention_decode
+    q, k, v, bt, sl = make([400, 3], 8, 1, seed=31)
+    k4, v4 = k.expand(-1, -1, 4, -1), v.expand(-1, -1, 4, -1)
+    out = paged_attention_decode(q, k4, v4, bt, sl, 400, 0.1)
+    ref, _, _, tol = reference(q, k, v, bt, sl, 0.1)
+    check(out, ref, tol)
+
+
+def test_own_workspace():
+    from starkv_b200.kernels.paged_attention import paged_attention_decode, workspace_bytes
+    q, k, v, bt, sl = make([5000, 200], 8, 2, seed=32)
+    ws = torch.empty(workspace_bytes(8, 2, 128, 5000), dtype=torch.uint8, device=q.device)
+    a = paged_attention_decode(q, k, v, bt, sl, 5000, 0.1, ws=ws)
+    assert torch.equal(a, paged_attention_decode(q, k, v, bt, sl, 5000, 0.1))
+    with pytest.raises(RuntimeError, match="workspace"):
+        paged_attention_decode(q, k, v, bt, sl, 5000, 0.1, ws=ws[:-16])

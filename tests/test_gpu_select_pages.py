@@ -221,3 +221,55 @@ def test_sparse_decode_is_the_attention_over_the_selected_pages():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("P", [200, 900, 9100])
+@pytest.mark.parametrize("kind", ["equal", "few values", "spread", "nan"])
+def test_every_way_to_the_border(P, kind):
+    """Few and many pages next to the border, equal pages, units longer than what is copied to
+    shared memory, NaN among them."""
+    from starkv_b200.kernels.paged_attention import select_pages
+    dev = cuda()
+    g = torch.Generator(device=dev).manual_seed(P)
+    a, c = (torch.randn(P + 1, 2, 64, generator=g, device=dev) for _ in range(2))
+    if kind == "equal":
+        a[:], c[:] = a[0].clone(), c[0].clone()
+    if kind == "few values":
+        pick = torch.randint(0, 3, (P + 1,), generator=g, device=dev)
+        a, c = a[:3][pick], c[:3][pick]
+    bounds = torch.stack([torch.minimum(a, c), torch.maximum(a, c)], 2).to(torch.bfloat16)
+    if kind == "nan":
+        bounds[torch.randint(1, P, (40,), generator=g, device=dev), 1, 0, 3] = float("nan")
+    q = torch.randn(2, 6, 64, generator=g, device=dev).to(torch.bfloat16)
+    bt = torch.arange(1, P + 1, device=dev, dtype=torch.int32).expand(2, P)      # one table row for both
+    sl = torch.tensor([P, P - 7], dtype=torch.int32, device=dev)
+    for top in (2, 30, 170):
+        got = select_pages(q, bounds, bt, sl, P, 1, top)
+        assert torch.equal(got.cpu(), expected(q, bounds, bt, sl.tolist(), 1, top, 1, 1)), top
+
+
+def test_two_selections_at_once():
+    from starkv_b200.kernels.paged_attention import sparse_paged_decode
+    import test_gpu_paged_attention as A
+    from starkv_b200.kernels.paged_attention import empty_bounds, update_page_bounds
+    graphs, outs, args = [], [], []
+    for seed, lens in ((40, [3000, 17, 900]), (41, [5, 2000, 2500])):
+        q, k, v, bt, sl = A.make(lens, 8, 2, seed=seed)
+        b = empty_bounds(k)
+        update_page_bounds(k, b, bt, sl, 3000, max_new=3000)
+        sparse_paged_decode(q, k, v, b, bt, sl, 3000, 0.1, 9)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(sparse_paged_decode(q, k, v, b, bt, sl, 3000, 0.1, 9))
+        args.append((q, k, v, b, bt, sl))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for (q, k, v, b, bt, sl), (out, pages) in zip(args, outs):
+        assert torch.equal(pages.cpu(), expected(q, b, bt, sl.tolist(), 16, 9, 1, 1))
+        ref, _, _, tol = A.reference(q, k, v, bt, sl, 0.1, pages=pages)
+        A.check(out, ref, tol)

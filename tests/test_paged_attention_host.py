@@ -35,10 +35,18 @@ def attend(q=None, k=None, v=None, bt=None, sl=None, **kw):
     (dict(pages=torch.zeros(2, 1, 3, dtype=torch.int32)), "pages must be"),
     (dict(out=torch.zeros(2, 4, 128)), "out must be"),
     (dict(), "one CUDA device"),
+    (dict(return_partial=True, partial=torch.zeros(8 * 130 - 1)), "at least 1040"),
+    (dict(return_partial=True, partial=torch.zeros(8 * 130, dtype=BF)), "f32 buffer"),
 ])
 def test_attention_refusals(kw, say):
     with pytest.raises(ValueError, match=say):
         attend(**kw)
+
+
+def test_attention_refuses_to_write_over_its_query():
+    q = torch.zeros(2, 4, 128, dtype=BF)
+    with pytest.raises(ValueError, match="query itself"):
+        attend(q=q, out=q)
 
 
 def test_select_and_bounds_refusals():
