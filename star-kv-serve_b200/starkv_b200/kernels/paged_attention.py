@@ -44,7 +44,8 @@ _CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}   # the cache's el
 
 def _tables(what: str, n: int, block_table: torch.Tensor, seq_lens: torch.Tensor):
     """(block_table, seq_lens) as int32, the lengths contiguous."""
-    if block_table.dim() != 2 or block_table.shape[0] != n or seq_lens.shape != (n,):
+    sizes = block_table.shape
+    if len(sizes) != 2 or sizes[0] != n or seq_lens.shape != (n,):
         raise ValueError(f"{what}: block_table must be [{n}, max_blocks] and seq_lens [{n}]")
     if block_table.dtype is not torch.int32:
         block_table = block_table.to(torch.int32)
@@ -53,14 +54,12 @@ def _tables(what: str, n: int, block_table: torch.Tensor, seq_lens: torch.Tensor
     return block_table, seq_lens
 
 
-def _cache_sizes(what: str, name: str, cache: torch.Tensor, dtype: torch.dtype):
-    """The sizes of a cache tensor, checked against the call's element type."""
-    sizes = cache.shape
-    if len(sizes) != 4 or sizes[3] not in HEAD_DIMS or cache.stride(3) != 1:
+def _refuse_cache(what: str, name: str, cache: torch.Tensor, dtype: torch.dtype) -> None:
+    """The error for a cache tensor that a call does not take, if it does not."""
+    if cache.dim() != 4 or cache.shape[3] not in HEAD_DIMS or cache.stride(3) != 1:
         raise ValueError(f"{what}: {name} must be [num_blocks, block_size, H_kv, 64 or 128], last dimension contiguous")
     if cache.dtype is not dtype or dtype not in _CODES:
         raise ValueError(f"{what}: all tensors must be bf16 or f16, the same as the cache")
-    return sizes
 
 
 def _query_sizes(what: str, query: torch.Tensor, num_kv_heads: int, head_dim: int):
@@ -113,9 +112,15 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
             ws, status, select=None):
     """The checks and the call of the attention; ``select`` = (bounds, sinks, recent): the
     pages are selected first, in the same call of the library."""
-    nb, bs, hkv, d = _cache_sizes(what, "k_cache", k_cache, query.dtype)
-    if _cache_sizes(what, "v_cache", v_cache, query.dtype) != k_cache.shape:
+    # short on purpose: at small batches the host's part of a call takes longer than the GPU's
+    dtype, sizes = query.dtype, k_cache.shape
+    ks, vs, qs = k_cache.stride(), v_cache.stride(), query.stride()
+    if dtype not in _CODES or len(sizes) != 4 or sizes[3] not in HEAD_DIMS or k_cache.dtype is not dtype \
+            or v_cache.dtype is not dtype or v_cache.shape != sizes or ks[3] != 1 or vs[3] != 1:
+        _refuse_cache(what, "k_cache", k_cache, dtype)
+        _refuse_cache(what, "v_cache", v_cache, dtype)
         raise ValueError(f"{what}: k_cache and v_cache must have the same shape")
+    nb, bs, hkv, d = sizes
     n, hq, _ = _query_sizes(what, query, hkv, d)
     block_table, seq_lens = _tables(what, n, block_table, seq_lens)
     top, pg = 0, (0, 0)
@@ -160,10 +165,9 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
         ws = seq_lens.new_empty((need + 3) // 4) if need else None
     P = _lib.addr
     a = _lib.pack_paged_attn(
-        query.data_ptr(), *query.stride()[:2], k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(),
-        *v_cache.stride()[:3], block_table.data_ptr(), *block_table.stride(), seq_lens.data_ptr(), P(pages), *pg,
-        out.data_ptr(), *out.stride()[:2], P(m), P(l), P(status), _CODES[query.dtype], n, hq, hkv, d, nb, bs,
-        block_table.shape[1], int(max_seq_len), top, float(scale))
+        query.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
+        block_table.data_ptr(), *block_table.stride(), seq_lens.data_ptr(), P(pages), *pg, out.data_ptr(),
+        *out.stride()[:2], P(m), P(l), P(status), _CODES[dtype], n, hq, hkv, d, nb, bs, block_table.shape[1], int(max_seq_len), top, float(scale))
     size = 0 if ws is None else ws.nbytes
     if select is None:
         _lib.launch(what, idx, _lib.lib().starkv_paged_attention, a, P(ws), size)
@@ -197,7 +201,8 @@ def update_page_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table:
     max_new=1 after a decode step, with the longest prompt after a prefill. Other pages'
     bounds stay as they are."""
     what = "update_page_bounds"
-    nb, bs, hkv, d = _cache_sizes(what, "k_cache", k_cache, k_cache.dtype)
+    _refuse_cache(what, "k_cache", k_cache, k_cache.dtype)
+    nb, bs, hkv, d = k_cache.shape
     if bounds.shape != (nb, hkv, 2, d) or bounds.dtype is not k_cache.dtype or bounds.stride(-1) != 1 \
             or bounds.stride(-2) != d:
         raise ValueError(f"{what}: bounds must be [{nb}, {hkv}, 2, {d}] in the cache's dtype, (lo, hi) contiguous")

@@ -13,41 +13,46 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .paged_attention import _CODES, HEAD_DIMS, _cache_sizes
+from .paged_attention import _CODES, HEAD_DIMS, _refuse_cache
 
-_Z2, _Z3 = (0, 0), (0, 0, 0)
+_Z3 = (0, 0, 0)
 
 
 _INDEX = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 _FLOAT = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
 
 
-def _rows(what: str, name: str, t: torch.Tensor, sizes, dtype) -> None:
-    if t.shape != sizes or t.dtype is not dtype or t.stride(2) != 1:
+def _rows(what: str, name: str, t: torch.Tensor, sizes, dtype):
+    """The strides of a [n, heads, head_dim] tensor, checked."""
+    st = t.stride()
+    if t.shape != sizes or t.dtype is not dtype or st[2] != 1:
         raise ValueError(f"{what}: {name} must be {list(sizes)} in the query's dtype, last dimension contiguous")
+    return st
 
 
 def _run(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping, q_weight, k_weight, eps, q_out, k_out,
          status):
-    q_sizes, dtype = q.shape, q.dtype
-    if len(q_sizes) != 3 or q_sizes[2] not in HEAD_DIMS or q_sizes[1] == 0 or q.stride(2) != 1:
+    # short on purpose: at small batches the host's part of a call takes longer than the GPU's
+    q_sizes, dtype, qs = q.shape, q.dtype, q.stride()
+    if len(q_sizes) != 3 or q_sizes[2] not in HEAD_DIMS or q_sizes[1] == 0 or qs[2] != 1:
         raise ValueError(f"{what}: q must be [n, heads, 64 or 128], last dimension contiguous")
     if dtype not in _CODES:
         raise ValueError(f"{what}: q, k and v must be bf16 or f16")
     n, hq, d = q_sizes
-    hkv = 0
+    hkv, ks, vs, os, kos = 0, _Z3, _Z3, _Z3, _Z3
     if k is not None:
         if k.dim() != 3 or k.shape[1] == 0:
             raise ValueError(f"{what}: k must be [n, KV heads, {d}]")
         hkv = k.shape[1]
         k_sizes = (n, hkv, d)
-        _rows(what, "k", k, k_sizes, dtype)
+        ks = _rows(what, "k", k, k_sizes, dtype)
     if positions.shape != (n,) or positions.dtype not in _INDEX:
         raise ValueError(f"{what}: positions must be int32 or int64 [{n}]")
     if cos_sin_cache.dim() != 2 or cos_sin_cache.dtype not in _FLOAT:
         raise ValueError(f"{what}: cos_sin_cache must be a bf16, f16 or f32 [positions, rot]")
     rows, rot = cos_sin_cache.shape
-    if cos_sin_cache.stride(1) != 1 or rot % 16 or not 0 < rot <= d:
+    cs = cos_sin_cache.stride()
+    if cs[1] != 1 or rot % 16 or not 0 < rot <= d:
         raise ValueError(f"{what}: cos_sin_cache must be [positions, rot], contiguous rows, rot a multiple of 16 and at "
                          f"most {d}")
     w_dtype = None
@@ -59,20 +64,26 @@ def _run(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping
                 raise ValueError(f"{what}: q_weight and k_weight must share one dtype")
             w_dtype = w.dtype
     nb = bs = slot_dtype = 0
+    kcs = vcs = _Z3
     if k_cache is not None:
-        nb, bs = _cache_sizes(what, "k_cache", k_cache, dtype)[:2]
-        if _cache_sizes(what, "v_cache", v_cache, dtype) != k_cache.shape or k_cache.shape[2:] != (hkv, d):
+        sizes, kcs, vcs = k_cache.shape, k_cache.stride(), v_cache.stride()
+        if len(sizes) != 4 or sizes[2:] != (hkv, d) or v_cache.shape != sizes or k_cache.dtype is not dtype \
+                or v_cache.dtype is not dtype or kcs[3] != 1 or vcs[3] != 1:
+            _refuse_cache(what, "k_cache", k_cache, dtype)
+            _refuse_cache(what, "v_cache", v_cache, dtype)
             raise ValueError(f"{what}: k_cache and v_cache must both be [num_blocks, block_size, {hkv}, {d}]")
-        _rows(what, "v", v, k_sizes, dtype)
+        vs = _rows(what, "v", v, k_sizes, dtype)
         if slot_mapping.shape != (n,) or slot_mapping.dtype not in _INDEX:
             raise ValueError(f"{what}: slot_mapping must be int32 or int64 [{n}]")
+        nb, bs = sizes[0], sizes[1]
         slot_mapping, slot_dtype = slot_mapping.contiguous(), _INDEX[slot_mapping.dtype]
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        os = (hq * d, d)
     else:
-        _rows(what, "q_out", q_out, q_sizes, dtype)
+        os = _rows(what, "q_out", q_out, q_sizes, dtype)
     if k_out is not None:
-        _rows(what, "k_out", k_out, k_sizes, dtype)
+        kos = _rows(what, "k_out", k_out, k_sizes, dtype)
     positions = positions.contiguous()
     idx = _lib.same_device(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping, q_weight, k_weight,
                            q_out, k_out, status)
@@ -80,13 +91,11 @@ def _run(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping
         return q_out
     P = _lib.addr
     a = _lib.pack_norm_rope(
-        q.data_ptr(), *q.stride()[:2], P(k), *(_Z2 if k is None else k.stride()[:2]),
-        P(v), *(_Z2 if v is None else v.stride()[:2]), q_out.data_ptr(), *q_out.stride()[:2],
-        P(k_out), *(_Z2 if k_out is None else k_out.stride()[:2]), P(q_weight), P(k_weight), positions.data_ptr(),
-        cos_sin_cache.data_ptr(), cos_sin_cache.stride(0), P(k_cache), *(_Z3 if k_cache is None else k_cache.stride()[:3]),
-        P(v_cache), *(_Z3 if v_cache is None else v_cache.stride()[:3]), P(slot_mapping), P(status), _CODES[dtype],
-        _FLOAT.get(w_dtype, 0), _INDEX[positions.dtype], _FLOAT[cos_sin_cache.dtype], slot_dtype, n, hq, hkv, d, rot,
-        rows, nb, bs, float(eps))
+        q.data_ptr(), qs[0], qs[1], P(k), ks[0], ks[1], P(v), vs[0], vs[1], q_out.data_ptr(), os[0], os[1],
+        P(k_out), kos[0], kos[1], P(q_weight), P(k_weight), positions.data_ptr(), cos_sin_cache.data_ptr(), cs[0],
+        P(k_cache), kcs[0], kcs[1], kcs[2], P(v_cache), vcs[0], vcs[1], vcs[2], P(slot_mapping), P(status),
+        _CODES[dtype], _FLOAT.get(w_dtype, 0), _INDEX[positions.dtype], _FLOAT[cos_sin_cache.dtype], slot_dtype, n, hq,
+        hkv, d, rot, rows, nb, bs, float(eps))
     _lib.launch(what, idx, _lib.lib().starkv_norm_rope, a)
     return q_out
 
