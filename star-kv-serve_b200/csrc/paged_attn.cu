@@ -170,9 +170,11 @@ __device__ __forceinline__ void store_out(const PagedAttnParams& p, int b, int h
   store4(reinterpret_cast<T*>(p.out) + at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
-// kTwo: more than 8 query heads in the unit's MMA rows. kThird: weights in three parts,
-// for the bf16 partial form, whose output is f32.
-template <typename T, int D, bool kTwo, bool kSparse, bool kThird>
+// kTwo: more than 8 query heads in the unit's MMA rows. kF32: the partial form, whose
+// output is f32 and shows what 16 bits hide: bf16 weights in three parts, and every MMA
+// adds to zero and the result to the sum with a rounded f32 addition, since the tensor
+// core's own accumulation cuts off (131071 tokens: 1.7e-6 off, relative in norm, that way).
+template <typename T, int D, bool kTwo, bool kSparse, bool kF32>
 __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttnParams p) {
   using R = Ring<D>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -185,6 +187,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   const uint32_t ring = smem_u32(smem) + warp * R::warp_bytes;
   const float c_log2 = p.scale * 1.4426950408889634f;
   constexpr float kBias = weight_bias<T>();
+  constexpr bool kThird = kF32 && std::is_same<T, __nv_bfloat16>::value;
 
   // the joining kernel's blocks may take the place of CTAs that are done; they wait for all
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -339,8 +342,19 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
         for (int kk = 0; kk < kKSteps; ++kk) {
           uint32_t r[4];
           ldsm4(a + (((2 * kk + (mi & 1)) ^ rr) << 4), r);
-          mma16816<T>(s0, qa[kk], r[0], r[1]);
-          mma16816<T>(s1, qa[kk], r[2], r[3]);
+          if (kF32) {
+            float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+            mma16816<T>(t0, qa[kk], r[0], r[1]);
+            mma16816<T>(t1, qa[kk], r[2], r[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s0[e] += t0[e];
+              s1[e] += t1[e];
+            }
+          } else {
+            mma16816<T>(s0, qa[kk], r[0], r[1]);
+            mma16816<T>(s1, qa[kk], r[2], r[3]);
+          }
         }
       }
       if (valid != 0xffffu) {
@@ -423,15 +437,25 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
         for (int j = 0; j < kKSteps; ++j) {
           uint32_t r[4];
           ldsm4_t(a + (((2 * j + (mi >> 1)) ^ rr) << 4), r);
-          mma16816<T>(o[2 * j], pa, r[0], r[1]);
-          mma16816<T>(o[2 * j + 1], pa, r[2], r[3]);
-          if (kTwo) {
-            mma16816<T>(o[2 * j], pl, r[0], r[1]);
-            mma16816<T>(o[2 * j + 1], pl, r[2], r[3]);
+          float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+          float(&x)[4] = kF32 ? t0 : o[2 * j];
+          float(&y)[4] = kF32 ? t1 : o[2 * j + 1];
+          if (kThird) {   // the smallest part first
+            mma16816<T>(x, pt, r[0], r[1]);
+            mma16816<T>(y, pt, r[2], r[3]);
           }
-          if (kThird) {
-            mma16816<T>(o[2 * j], pt, r[0], r[1]);
-            mma16816<T>(o[2 * j + 1], pt, r[2], r[3]);
+          if (kTwo) {
+            mma16816<T>(x, pl, r[0], r[1]);
+            mma16816<T>(y, pl, r[2], r[3]);
+          }
+          mma16816<T>(x, pa, r[0], r[1]);
+          mma16816<T>(y, pa, r[2], r[3]);
+          if (kF32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              o[2 * j][e] += t0[e];
+              o[2 * j + 1][e] += t1[e];
+            }
           }
         }
       }
@@ -608,11 +632,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttnParam
 }
 
 template <typename T, int D, bool kSparse>
-const void* attn_fn(bool two, bool third) {
-  constexpr bool k3 = std::is_same<T, __nv_bfloat16>::value;
-  if (third)
-    return two ? (const void*)paged_attn_kernel<T, D, true, kSparse, k3>
-               : (const void*)paged_attn_kernel<T, D, false, kSparse, k3>;
+const void* attn_fn(bool two, bool f32) {
+  if (f32)
+    return two ? (const void*)paged_attn_kernel<T, D, true, kSparse, true>
+               : (const void*)paged_attn_kernel<T, D, false, kSparse, true>;
   return two ? (const void*)paged_attn_kernel<T, D, true, kSparse, false>
              : (const void*)paged_attn_kernel<T, D, false, kSparse, false>;
 }
@@ -620,9 +643,8 @@ const void* attn_fn(bool two, bool third) {
 template <typename T, int D>
 int launch_typed(const PagedAttnParams& p, int num_sms, cudaStream_t stream) {
   const bool two = p.group > 8;
-  // f16 parts hold 22 bits, as much as f32 sums need
-  const bool third = p.m_out && std::is_same<T, __nv_bfloat16>::value;
-  const void* fn = p.pages ? attn_fn<T, D, true>(two, third) : attn_fn<T, D, false>(two, third);
+  const bool f32 = p.m_out != nullptr;
+  const void* fn = p.pages ? attn_fn<T, D, true>(two, f32) : attn_fn<T, D, false>(two, f32);
   const int smem = Ring<D>::bytes;
   if (const int st = allow_smem(fn, smem)) return st;
   PagedAttnParams q = p;
