@@ -60,10 +60,10 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) bounds_kernel(const PageBoundsParams p) {
   constexpr int kChunks = D / 8, kRowsPer = 32 / kChunks;
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int hk = (int)(item % p.num_kv_heads);
-  const int64_t bp = item / p.num_kv_heads;
-  const int b = (int)(bp / p.max_pages), j = (int)(bp % p.max_pages);
+  const unsigned item = blockIdx.x * kWarps + (threadIdx.x >> 5);   // 64-bit divisions would show
+  const unsigned bp = item / p.num_kv_heads;
+  const int hk = (int)(item - bp * p.num_kv_heads);
+  const int b = (int)(bp / p.max_pages), j = (int)(bp - b * p.max_pages);
   if (b >= p.n) return;
   const int L = min(max(p.seq_lens[b], 0), p.max_len);
   const int fresh = p.new_lens ? min(max(p.new_lens[b], 0), p.max_new) : p.max_new;
@@ -777,7 +777,7 @@ template <typename T, int D>
 int launch_bounds_typed(PageBoundsParams p, cudaStream_t stream) {
   const int64_t items = (int64_t)p.n * p.max_pages * p.num_kv_heads;
   const int64_t blocks = (items + kWarps - 1) / kWarps;
-  if (blocks > 0x7fffffff) return STARKV_EINVAL;
+  if (items > 0x7fffffff) return STARKV_EINVAL;
   void* args[] = {&p};
   return cudaLaunchKernel((const void*)bounds_kernel<T, D>, dim3((unsigned)blocks), dim3(kThreads), args, 0, stream) ==
                  cudaSuccess
