@@ -65,7 +65,7 @@ LENS = [0, 1, 16, 17, 127, 128, 129, 145, 1000, 5000]
 
 
 @pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 128), (torch.bfloat16, 64)])
-@pytest.mark.parametrize("H,Hkv", [(4, 4), (8, 2), (5, 1)])
+@pytest.mark.parametrize("H,Hkv", [(4, 4), (8, 2), (5, 1), (6, 3), (11, 11), (40, 20)])
 def test_selection_at_edge_lengths(H, Hkv, dtype, D):
     run(LENS, H, Hkv, D=D, dtype=dtype, seed=H)
 
