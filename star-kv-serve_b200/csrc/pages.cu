@@ -178,18 +178,124 @@ constexpr int kRun = 16;     // pages of a run
 constexpr int kBatch = 32;   // block ids that a warp holds
 constexpr int kStep = 4;     // pages of a lane's step
 constexpr int kRing = 3;     // steps in the copies' ring
-constexpr int kRingBytes = kRing * kStep * 16 * kThreads;
+constexpr int ring_bytes(int threads) { return kRing * kStep * 16 * threads; }
+
+// Keys of the f32 scores of the competing pages i0 .. i1 - 1 of a (sequence, KV head), by one
+// warp of a CTA of kThr threads, to keys[i]; returns the scores' error, and the smallest and
+// the largest key.
+template <typename T, int D, int kThr>
+__device__ float score_pages(const SelectPagesParams& p, int b, int hk, int i0, int i1, uint8_t* ring, uint32_t* keys,
+                             uint32_t& k_lo, uint32_t& k_hi) {
+  constexpr int LP = 2 * D / 8;                      // lanes of one page's bounds
+  constexpr int kPer = kStep * (32 / LP);            // pages of a warp's step
+  constexpr int kSteps = kBatch / kPer;              // steps of a batch of block ids
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int e = lane % LP, sub = lane / LP;
+  const int d = (e * 8) % D;
+  const bool upper = e * 8 >= D;
+  const int steps = (i1 - i0 + kPer - 1) / kPer;
+  const int32_t* bt = p.block_table + b * p.bt_s0 + (int64_t)p.sinks * p.bt_s1;
+  const T* bounds = reinterpret_cast<const T*>(p.bounds) + (int64_t)hk * p.b_s1 + e * 8;
+  // A lane copies its own 16 bytes of a page into its own slots of the ring (cp.async,
+  // two steps ahead): no barrier between copy and use. Block ids come 32 at a time.
+  const uint32_t slots = smem_u32(ring) + tid * 16;
+  auto blocks_from = [&](int i) {   // lane l: the block of competing page i + l
+    int blk = bt[(int64_t)min(i + lane, i1 - 1) * p.bt_s1];   // past the end: the last page once more
+    if ((unsigned)blk >= (unsigned)p.num_blocks) {
+      record_status(p.status, STARKV_EBOUNDS);
+      blk = 0;
+    }
+    return blk;
+  };
+  int cur = 0, nxt = blocks_from(i0);
+  auto issue = [&](int j) {
+    if (j % kSteps == 0) {
+      cur = nxt;
+      nxt = blocks_from(i0 + (j / kSteps + 1) * kBatch);
+    }
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) {
+      const int blk = __shfl_sync(~0u, cur, j % kSteps * kPer + sub * kStep + u);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + (j % kRing * kStep + u) * kThr * 16),
+                   "l"(bounds + (int64_t)blk * p.b_s0)
+                   : "memory");
+    }
+  };
+  // the queries before the copies, so that they do not wait behind them
+  float w[8];
+  query_side(reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group) * p.q_s1 + d, p.q_s1, p.group,
+             upper, w);
+  float size = 0.f;                                // sum of |w| of this lane's channels
+#pragma unroll
+  for (int i = 0; i < 8; ++i) size += fabsf(w[i]);
+#pragma unroll
+  for (int j = 0; j < kRing - 1; ++j) {
+    if (j < steps) issue(j);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  k_lo = ~0u;
+  k_hi = 0;
+  uint32_t largest = 0;                            // largest |bound| of this lane's channels, as a pair
+      for (int j = 0; j < steps; ++j) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+    if (j + kRing - 1 < steps) issue(j + kRing - 1);   // into the slots of step j - 1
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    float s[kStep];
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) {
+      const uint4 v = *reinterpret_cast<const uint4*>(ring + ((j % kRing * kStep + u) * kThr + tid) * 16);
+      float f[8];
+      to_f32x8(T{}, v, f);
+      float2 a = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a = fma2(make_float2(f[2 * i], f[2 * i + 1]), make_float2(w[2 * i], w[2 * i + 1]), a);
+      s[u] = a.x + a.y;
+      largest = max_abs2(T{}, max_abs2(T{}, max_abs2(T{}, largest, v.x), v.y), max_abs2(T{}, v.z, v.w));
+    }
+    // sums over the LP lanes of a page: first steps that also halve the pages a lane holds
+    int at = j * kPer + sub * kStep, o = LP / 2;
+#pragma unroll
+    for (int h = kStep / 2; h >= 1; h >>= 1, o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < h; ++i) {
+        const float give = lane & o ? s[i] : s[i + h], keep = lane & o ? s[i + h] : s[i];
+        s[i] = keep + __shfl_xor_sync(~0u, give, o);
+      }
+      at += lane & o ? h : 0;
+    }
+    const int last = o;                            // lanes below: copies of the same page
+#pragma unroll
+    for (; o; o >>= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
+    if ((lane & (2 * last - 1)) == 0 && i0 + at < i1) {
+      const uint32_t k = order_key(s[0]);
+      keys[i0 + at] = k;
+      k_lo = min(k_lo, k);
+      k_hi = max(k_hi, k);
+    }
+  }
+  // Error of these scores: a term passes at most G - 1 roundings of 2^-24 in its weight
+  // (of terms of one sign), 5 in the lane and 5 between lanes, so (G + 9) 2^-24
+  // sum |w b| <= (G + 9) 2^-24 sum_lanes largest * size; 1.125 times (G + 11) covers the
+  // roundings of the bound itself.
+  float err;
+  {
+    float f[8];
+    to_f32x8(T{}, make_uint4(largest, 0, 0, 0), f);
+    err = fmaxf(fabsf(f[0]), fabsf(f[1])) * size;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) err += __shfl_xor_sync(~0u, err, o);   // D = 64: both halves, an upper bound
+    err *= 1.125f / (1 << 24) * (p.group + 11);
+  }
+  k_lo = __reduce_min_sync(~0u, k_lo);
+  k_hi = __reduce_max_sync(~0u, k_hi);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  return err;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesParams p) {
   extern __shared__ __align__(16) uint8_t ring[];
-  constexpr int LP = 2 * D / 8;                      // lanes of one page's bounds
-  constexpr int kPer = kStep * (32 / LP);            // pages of a warp's step
-  constexpr int kSteps = kBatch / kPer;              // steps of a batch of block ids
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int e = lane % LP, sub = lane / LP;
-  const int d = (e * 8) % D;
-  const bool upper = e * 8 >= D;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // pick_kernel waits for all of this one
   // The warps of a CTA take the same pages of up to eight KV heads, whose bounds lie side by
   // side: 4 KB of a page are read together where a warp alone reads 512 bytes.
@@ -213,104 +319,11 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
     const int here = min(runs - run, g1 - g);
     const int hk = min(group * abreast + warp % abreast, p.num_kv_heads - 1);   // the last group: the last head again
     const int i0 = run * kRun, i1 = min(i0 + here * kRun, N);   // competing pages i0 .. i1 - 1
-    const int steps = (i1 - i0 + kPer - 1) / kPer;
-    const int32_t* bt = p.block_table + b * p.bt_s0 + (int64_t)p.sinks * p.bt_s1;
-    const T* bounds = reinterpret_cast<const T*>(p.bounds) + (int64_t)hk * p.b_s1 + e * 8;
-    // A lane copies its own 16 bytes of a page into its own slots of the ring (cp.async,
-    // two steps ahead): no barrier between copy and use. Block ids come 32 at a time.
-    const uint32_t slots = smem_u32(ring) + tid * 16;
-    auto blocks_from = [&](int i) {   // lane l: the block of competing page i + l
-      int blk = bt[(int64_t)min(i + lane, i1 - 1) * p.bt_s1];   // past the end: the last page once more
-      if ((unsigned)blk >= (unsigned)p.num_blocks) {
-        record_status(p.status, STARKV_EBOUNDS);
-        blk = 0;
-      }
-      return blk;
-    };
-    int cur = 0, nxt = blocks_from(i0);
-    auto issue = [&](int j) {
-      if (j % kSteps == 0) {
-        cur = nxt;
-        nxt = blocks_from(i0 + (j / kSteps + 1) * kBatch);
-      }
-#pragma unroll
-      for (int u = 0; u < kStep; ++u) {
-        const int blk = __shfl_sync(~0u, cur, j % kSteps * kPer + sub * kStep + u);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + (j % kRing * kStep + u) * kThreads * 16),
-                     "l"(bounds + (int64_t)blk * p.b_s0)
-                     : "memory");
-      }
-    };
-    // the queries before the copies, so that they do not wait behind them
-    float w[8];
-    query_side(reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group) * p.q_s1 + d, p.q_s1, p.group,
-               upper, w);
-    float size = 0.f;                                // sum of |w| of this lane's channels
-#pragma unroll
-    for (int i = 0; i < 8; ++i) size += fabsf(w[i]);
-#pragma unroll
-    for (int j = 0; j < kRing - 1; ++j) {
-      if (j < steps) issue(j);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    uint32_t k_lo = ~0u, k_hi = 0;
-    uint32_t largest = 0;                            // largest |bound| of this lane's channels, as a pair
-    uint32_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride + i0;
-    for (int j = 0; j < steps; ++j) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
-      if (j + kRing - 1 < steps) issue(j + kRing - 1);   // into the slots of step j - 1
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      float s[kStep];
-#pragma unroll
-      for (int u = 0; u < kStep; ++u) {
-        const uint4 v = *reinterpret_cast<const uint4*>(ring + ((j % kRing * kStep + u) * kThreads + tid) * 16);
-        float f[8];
-        to_f32x8(T{}, v, f);
-        float2 a = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a = fma2(make_float2(f[2 * i], f[2 * i + 1]), make_float2(w[2 * i], w[2 * i + 1]), a);
-        s[u] = a.x + a.y;
-        largest = max_abs2(T{}, max_abs2(T{}, max_abs2(T{}, largest, v.x), v.y), max_abs2(T{}, v.z, v.w));
-      }
-      // sums over the LP lanes of a page: first steps that also halve the pages a lane holds
-      int at = j * kPer + sub * kStep, o = LP / 2;
-#pragma unroll
-      for (int h = kStep / 2; h >= 1; h >>= 1, o >>= 1) {
-#pragma unroll
-        for (int i = 0; i < h; ++i) {
-          const float give = lane & o ? s[i] : s[i + h], keep = lane & o ? s[i + h] : s[i];
-          s[i] = keep + __shfl_xor_sync(~0u, give, o);
-        }
-        at += lane & o ? h : 0;
-      }
-      const int last = o;                            // lanes below: copies of the same page
-#pragma unroll
-      for (; o; o >>= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
-      if ((lane & (2 * last - 1)) == 0 && i0 + at < i1) {
-        const uint32_t k = order_key(s[0]);
-        keys[at] = k;
-        k_lo = min(k_lo, k);
-        k_hi = max(k_hi, k);
-      }
-    }
-    // Error of these scores: a term passes at most G - 1 roundings of 2^-24 in its weight
-    // (of terms of one sign), 5 in the lane and 5 between lanes, so (G + 9) 2^-24
-    // sum |w b| <= (G + 9) 2^-24 sum_lanes largest * size; 1.125 times (G + 11) covers the
-    // roundings of the bound itself.
-    float err;
-    {
-      float f[8];
-      to_f32x8(T{}, make_uint4(largest, 0, 0, 0), f);
-      err = fmaxf(fabsf(f[0]), fabsf(f[1])) * size;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) err += __shfl_xor_sync(~0u, err, o);   // D = 64: both halves, an upper bound
-      err *= 1.125f / (1 << 24) * (p.group + 11);
-    }
-    k_lo = __reduce_min_sync(~0u, k_lo);
-    k_hi = __reduce_max_sync(~0u, k_hi);
+    uint32_t k_lo, k_hi;
+    const float err = score_pages<T, D, kThreads>(p, b, hk, i0, i1, ring,
+                                                  p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride, k_lo, k_hi);
     uint4* about = p.runs + ((int64_t)b * p.num_kv_heads + hk) * p.run_stride + run;
     for (int r = lane; r < here; r += 32) about[r] = make_uint4(__float_as_uint(err), k_lo, k_hi, 0);
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     g += here;
     run = 0;
     if (g < g1 && ++group == groups) {
@@ -326,6 +339,7 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
 constexpr int kPickWarpsMost = 32;
 constexpr int kAhead = 4;         // keys in flight per thread
 constexpr int kPickCache = 8192;  // keys that are copied to shared memory
+constexpr int kFusedPages = 512, kFusedThreads = 512;   // pages that pick_kernel scores itself
 
 constexpr int kBins = 2048;
 constexpr int kNear = 256;        // pages next to the border that are scored again one by one
@@ -461,12 +475,14 @@ __device__ void write_selected(int N, PickShared& sh, const Cls& cls, int rest, 
   }
 }
 
+// kFused: it scores the unit's pages itself (launch_select_typed says when).
 // kThr: 256 threads where the units fill the GPU (four CTAs to an SM), 1024 where they do
 // not and a unit's passes over many keys are the time (8192 pages: 20.9 -> 13.2 us).
-template <typename T, int D, int kThr>
+template <typename T, int D, int kThr, bool kFused>
 __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPagesParams p) {
   __shared__ PickShared sh;
-  __shared__ uint32_t cache[kPickCache];
+  constexpr int kCache = kFused ? kFusedPages : kPickCache;
+  __shared__ uint32_t cache[kCache];
   const int unit = blockIdx.x;
   const int hk = unit % p.num_kv_heads, b = unit / p.num_kv_heads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -481,7 +497,9 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
     for (int i = tid; i < p.recent; i += kThr) out[p.top - p.recent + i] = P - p.recent + i;
   }
   constexpr int LP = 2 * D / 8;
-  if (N > 0 && warp == 0) {   // for the scores in 64 bits, should there be any: before the wait it costs nothing
+  // for the scores in 64 bits, should there be any: before the wait it costs nothing, and the
+  // last warp has the fewest pages to score
+  if (N > 0 && warp == (kFused ? kThr / 32 - 1 : 0)) {
     const int d = (lane % LP * 8) % D;
     double w[8];
     query_side(reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group) * p.q_s1 + d, p.q_s1, p.group,
@@ -490,34 +508,44 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
     for (int i = 0; i < 8; ++i) sh.side[lane % LP * 8 + i] = w[i];
   }
   for (int i = tid; i < kBins / 4; i += kThr) sh.bins[i] = make_uint4(0, 0, 0, 0);
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // the scores are written
-  if (N == 0) return;
-  out += p.sinks;
-
-  // what the runs say: the largest error, smallest and largest key
+  // keys of the scores, their largest error, smallest and largest key
   uint32_t* keys = p.keys + (int64_t)unit * p.key_stride;
-  const uint4* runs = p.runs + (int64_t)unit * p.run_stride;
-  const int n_runs = (N + kRun - 1) / kRun;
   uint32_t k_lo = ~0u, k_hi = 0, e_bits = 0;
-  uint4 about = runs[min(tid, n_runs - 1)];
-  if (N <= kPickCache) {
-    for (int i = tid; i < N; i += 2 * kAhead * kThr) {
-      uint32_t k[2 * kAhead];
-#pragma unroll
-      for (int u = 0; u < 2 * kAhead; ++u) k[u] = keys[min(i + u * kThr, N - 1)];
-#pragma unroll
-      for (int u = 0; u < 2 * kAhead; ++u)
-        if (i + u * kThr < N) cache[i + u * kThr] = k[u];
-    }
+  if (kFused) {   // launched behind all earlier work, N <= kFusedPages
+    extern __shared__ __align__(16) uint8_t ring[];
+    if (N == 0) return;
     keys = cache;
+    const int per = ((N + kThr / 32 - 1) / (kThr / 32) + 7) & ~7;
+    if (warp * per < N)
+      e_bits = __float_as_uint(score_pages<T, D, kThr>(p, b, hk, warp * per, min((warp + 1) * per, N), ring, cache, k_lo,
+                                                       k_hi)) &
+               0x7fffffffu;
+  } else {
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the scores are written
+    if (N == 0) return;
+    const uint4* runs = p.runs + (int64_t)unit * p.run_stride;
+    const int n_runs = (N + kRun - 1) / kRun;
+    uint4 about = runs[min(tid, n_runs - 1)];
+    if (N <= kCache) {
+      for (int i = tid; i < N; i += 2 * kAhead * kThr) {
+        uint32_t k[2 * kAhead];
+#pragma unroll
+        for (int u = 0; u < 2 * kAhead; ++u) k[u] = keys[min(i + u * kThr, N - 1)];
+#pragma unroll
+        for (int u = 0; u < 2 * kAhead; ++u)
+          if (i + u * kThr < N) cache[i + u * kThr] = k[u];
+      }
+      keys = cache;
+    }
+    for (int r = tid;;) {
+      e_bits = max(e_bits, about.x & 0x7fffffffu);   // >= 0 or NaN: ordered as integers
+      k_lo = min(k_lo, about.y);
+      k_hi = max(k_hi, about.z);
+      if ((r += kThr) >= n_runs) break;
+      about = runs[r];
+    }
   }
-  for (int r = tid;;) {
-    e_bits = max(e_bits, about.x & 0x7fffffffu);     // >= 0 or NaN: ordered as integers
-    k_lo = min(k_lo, about.y);
-    k_hi = max(k_hi, about.z);
-    if ((r += kThr) >= n_runs) break;
-    about = runs[r];
-  }
+  out += p.sinks;
   e_bits = __reduce_max_sync(~0u, e_bits);
   k_lo = __reduce_min_sync(~0u, k_lo);
   k_hi = __reduce_max_sync(~0u, k_hi);
@@ -590,7 +618,7 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
 
   // ---- ordinary scores: one histogram of 2048 equal parts of the keys' range, then the few
   // pages of the border's part, and those within reach of it, one by one ----
-  if (N <= kPickCache && k_hi < ~0u && reach < INFINITY) {
+  if (N <= kCache && k_hi < ~0u && reach < INFINITY) {
     uint32_t* bins = reinterpret_cast<uint32_t*>(sh.bins);
     const int s = max(0, 21 - __clz(k_hi - k_lo));   // (k_hi - k_lo) >> s < 2048
     for (int i = tid; i < N; i += kThr) atomicAdd(&bins[(keys[i] - k_lo) >> s], 1u);
@@ -751,25 +779,35 @@ int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
   p.runs = reinterpret_cast<uint4*>(p.scratch);
   p.exact = reinterpret_cast<uint64_t*>(p.runs + units * p.run_stride);
   p.keys = reinterpret_cast<uint32_t*>(p.exact + units * p.key_stride);
-  const void* fn = (const void*)score_kernel<T, D>;
-  if (const int st = allow_smem(fn, kRingBytes)) return st;
   void* args[] = {&p};
-  if (p.key_stride > p.top) {   // else no sequence has pages to choose from
-    const int64_t grid = std::min<int64_t>(3 * num_sms, units * p.run_stride);
-    if (cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), args, kRingBytes, stream) != cudaSuccess)
-      return STARKV_ECUDA;
-  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)units);
-  const bool few = units <= num_sms && p.key_stride > 1024;   // 281 pages: 11.0 against 12.1 us with 1024 threads
-  cfg.blockDim = dim3(few ? 1024 : 256);
   cfg.stream = stream;
   cfg.attrs = attr;
+  // One kernel where a CTA per unit, one to an SM, is enough for the reads (8 units of 256 /
+  // 512 / 1024 pages: 13.6 / 16 / 20.6 us against 14.2 / 14.3 / 14.4 in two, 32 units of 281
+  // small pages 15.1 against 17.7; and a launch less, 4 us of the host's time).
+  if (units <= num_sms && p.key_stride <= kFusedPages) {
+    const void* fn = (const void*)pick_kernel<T, D, kFusedThreads, true>;
+    if (const int st = allow_smem(fn, ring_bytes(kFusedThreads))) return st;
+    cfg.blockDim = dim3(kFusedThreads);
+    cfg.dynamicSmemBytes = ring_bytes(kFusedThreads);
+    return cudaLaunchKernelExC(&cfg, fn, args) == cudaSuccess ? STARKV_OK : STARKV_ECUDA;
+  }
+  if (p.key_stride > p.top) {   // else no sequence has pages to choose from
+    const void* fn = (const void*)score_kernel<T, D>;
+    if (const int st = allow_smem(fn, ring_bytes(kThreads))) return st;
+    const int64_t grid = std::min<int64_t>(3 * num_sms, units * p.run_stride);
+    if (cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), args, ring_bytes(kThreads), stream) != cudaSuccess)
+      return STARKV_ECUDA;
+  }
+  const bool few = units <= num_sms && p.key_stride > 1024;
+  cfg.blockDim = dim3(few ? 1024 : 256);
   cfg.numAttrs = p.key_stride > p.top;   // behind score_kernel alone may the launch come early
-  const void* pick = few ? (const void*)pick_kernel<T, D, 1024> : (const void*)pick_kernel<T, D, 256>;
+  const void* pick = few ? (const void*)pick_kernel<T, D, 1024, false> : (const void*)pick_kernel<T, D, 256, false>;
   return cudaLaunchKernelExC(&cfg, pick, args) == cudaSuccess ? STARKV_OK : STARKV_ECUDA;
 }
 

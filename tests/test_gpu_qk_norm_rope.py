@@ -160,3 +160,42 @@ def test_captured():
     torch.cuda.synchronize()
     close(out, formula(qkv[:, :4], w, cs, pos, 1e-6))
     assert torch.equal(vc.view(-1, 2, 128)[30:50], qkv[:, 6:])
+
+
+def test_write_in_place_and_empty():
+    from starkv_b200.kernels.qk_norm_rope import qk_norm_rope_write
+    qkv, w, pos = inputs(300, 8, 2, 128, torch.bfloat16, seed=12)
+    dev = qkv.device
+    cs = rotary_table(500, 128, torch.bfloat16, dev)
+    kc, vc = torch.zeros(2, 20, 16, 2, 128, dtype=torch.bfloat16, device=dev).unbind(0)
+    slots = torch.randperm(320, device=dev)[:300]
+    q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:].clone()
+    want = formula(q, w, cs, pos, 1e-6), formula(k, w, cs, pos, 1e-6)
+    got = qk_norm_rope_write(q, k, qkv[:, 10:], pos, cs, kc, vc, slots, q_weight=w, k_weight=w, q_out=q, k_out=k)
+    assert got.data_ptr() == qkv.data_ptr()
+    close(qkv[:, :8], want[0])
+    close(qkv[:, 8:10], want[1])
+    assert torch.equal(qkv[:, 10:], v)
+    assert torch.equal(kc.view(320, 2, 128)[slots], qkv[:, 8:10]) and torch.equal(vc.view(320, 2, 128)[slots], v)
+    before = kc.clone()
+    none = qk_norm_rope_write(q[:0], k[:0], v[:0], pos[:0], cs, kc, vc, slots[:0])
+    assert none.shape == (0, 8, 128) and torch.equal(kc, before)
+
+
+@pytest.mark.parametrize("H,Hkv,n", [(32, 8, 1000), (7, 3, 2000), (1, 1, 9000), (33, 17, 700), (64, 64, 150)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_batches_of_odd_heads(H, Hkv, n, D):
+    """Batches that take the kernel's several-steps form, head counts that leave a step partly
+    empty, one norm given and the other not."""
+    from starkv_b200.kernels.qk_norm_rope import qk_norm_rope_write
+    qkv, w, pos = inputs(n, H, Hkv, D, torch.float16, seed=H)
+    dev = qkv.device
+    cs = rotary_table(500, D, torch.float32, dev)
+    kc, vc = torch.zeros(2, -(-n // 16), 16, Hkv, D, dtype=torch.float16, device=dev).unbind(0)
+    slots = torch.arange(n, device=dev)
+    q, k, v = qkv[:, :H], qkv[:, H:H + Hkv], qkv[:, H + Hkv:]
+    for qw, kw in ((w, None), (None, w)):
+        got = qk_norm_rope_write(q, k, v, pos, cs, kc, vc, slots, q_weight=qw, k_weight=kw)
+        close(got, formula(q, qw, cs, pos, 1e-6))
+        close(kc.view(-1, Hkv, D)[:n], formula(k, kw, cs, pos, 1e-6))
+        assert torch.equal(vc.view(-1, Hkv, D)[:n], v)

@@ -34,7 +34,8 @@ def expected(q, bounds, bt, lens, bs, top, sinks, recent):
             s = torch.maximum(Q[:, None] * B[:, 0], Q[:, None] * B[:, 1]).sum((0, 2))
             s = torch.where(s.isnan(), float("inf"), s)
             keep = list(range(sinks)) + list(range(P - recent, P))
-            rest = [i for i in torch.argsort(s, descending=True, stable=True).tolist() if i not in set(keep)]
+            kept = set(keep)
+            rest = [i for i in torch.argsort(s, descending=True, stable=True).tolist() if i not in kept]
             out[b, h] = torch.tensor(sorted(keep + rest[:top - len(keep)]), dtype=torch.int32)
     return out
 
@@ -223,11 +224,12 @@ def test_sparse_decode_is_the_attention_over_the_selected_pages():
     assert torch.equal(again, out)
 
 
-@pytest.mark.parametrize("P", [200, 900, 9100])
+@pytest.mark.parametrize("P,n", [(200, 2), (500, 2), (900, 2), (2100, 2), (9100, 2), (40, 80), (900, 80)])
 @pytest.mark.parametrize("kind", ["equal", "few values", "spread", "nan"])
-def test_every_way_to_the_border(P, kind):
-    """Few and many pages next to the border, equal pages, units longer than what is copied to
-    shared memory, NaN among them."""
+def test_every_way_to_the_border(P, n, kind):
+    """Few and many pages next to the border, equal pages, NaN among them; units that are
+    scored in one kernel with the selection (few, up to 512 pages) and in two (long ones,
+    also longer than what is copied to shared memory, and more units than SMs)."""
     from starkv_b200.kernels.paged_attention import select_pages
     dev = cuda()
     g = torch.Generator(device=dev).manual_seed(P)
@@ -240,9 +242,9 @@ def test_every_way_to_the_border(P, kind):
     bounds = torch.stack([torch.minimum(a, c), torch.maximum(a, c)], 2).to(torch.bfloat16)
     if kind == "nan":
         bounds[torch.randint(1, P, (40,), generator=g, device=dev), 1, 0, 3] = float("nan")
-    q = torch.randn(2, 6, 64, generator=g, device=dev).to(torch.bfloat16)
-    bt = torch.arange(1, P + 1, device=dev, dtype=torch.int32).expand(2, P)      # one table row for both
-    sl = torch.tensor([P, P - 7], dtype=torch.int32, device=dev)
+    q = torch.randn(n, 6, 64, generator=g, device=dev).to(torch.bfloat16)
+    bt = torch.arange(1, P + 1, device=dev, dtype=torch.int32).expand(n, P)      # one table row for all
+    sl = torch.tensor([P, P - 7] * (n // 2), dtype=torch.int32, device=dev)
     for top in (2, 30, 170):
         got = select_pages(q, bounds, bt, sl, P, 1, top)
         assert torch.equal(got.cpu(), expected(q, bounds, bt, sl.tolist(), 1, top, 1, 1)), top
@@ -273,3 +275,29 @@ def test_two_selections_at_once():
         assert torch.equal(pages.cpu(), expected(q, b, bt, sl.tolist(), 16, 9, 1, 1))
         ref, _, _, tol = A.reference(q, k, v, bt, sl, 0.1, pages=pages)
         A.check(out, ref, tol)
+
+
+def test_given_outputs_strided_bounds_and_empty_batches():
+    from starkv_b200.kernels.paged_attention import select_pages, sparse_paged_decode, update_page_bounds
+    import test_gpu_paged_attention as A
+    q, k, v, bt, sl = A.make([900, 20], 4, 2, seed=50)
+    wide = torch.full((k.shape[0], 3, 2, 128), 5.0, dtype=k.dtype, device=k.device)
+    bounds = wide[:, :2]
+    update_page_bounds(k, bounds, bt.long(), sl.long(), 900, max_new=900)
+    assert (wide[:, 2] == 5).all()
+    both = torch.full((2, 2, 2, 7), -9, dtype=torch.int32, device=k.device)
+    lens = torch.stack([sl, sl + 1], 1)[:, 0]                   # a strided view
+    got = select_pages(q, bounds, bt, lens, 900, 16, 7, out=both[:, 1])
+    assert got.data_ptr() == both[:, 1].data_ptr() and (both[:, 0] == -9).all()
+    assert torch.equal(got.cpu(), expected(q, bounds, bt, sl.tolist(), 16, 7, 1, 1))
+    out, pages = sparse_paged_decode(q, k, v, bounds, bt, lens, 900, 0.1, 7)
+    assert torch.equal(pages, got)
+    ref, _, _, tol = A.reference(q, k, v, bt, sl, 0.1, pages=pages)
+    A.check(out, ref, tol)
+    assert select_pages(q[:0], bounds, bt[:0], sl[:0], 900, 16, 7).shape == (0, 2, 7)
+    out, pages = sparse_paged_decode(q[:0], k, v, bounds, bt[:0], sl[:0], 900, 0.1, 7)
+    assert out.shape == (0, 4, 128) and pages.shape == (0, 2, 7)
+    before = wide.clone()
+    update_page_bounds(k, bounds, bt[:0], sl[:0], 900)
+    update_page_bounds(k, bounds, bt, sl, 900, max_new=0)
+    assert torch.equal(wide, before)
