@@ -18,11 +18,11 @@
 // f32 and also bounds the error, and pick_kernel sums again in 64 bits only the pages
 // that lie within the error of the border, mostly none.
 //
-// score_kernel takes the batch's pages in runs of 16, an equal number of runs per warp
+// score_kernel takes the batch's pages in runs of 16, an equal number of runs per CTA
 // whatever the mix of lengths, and writes order-preserving keys. pick_kernel takes a CTA
 // per (sequence, KV head) and finds the border by radix selection from the highest bit in
 // which the unit's keys differ (one or two passes of 8 bits on real scores). Ties go to
-// the lowest page.
+// the lowest page. Few units of few pages: pick_kernel scores them itself (kFused).
 #include <algorithm>
 #include <type_traits>
 
@@ -155,12 +155,18 @@ template <typename T, typename W>
 __device__ __forceinline__ void query_side(const T* q, int64_t stride, int group, bool upper, W (&w)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 0;
-#pragma unroll 4
-  for (int h = 0; h < group; ++h) {
-    float f[8];
-    to_f32x8(T{}, *reinterpret_cast<const uint4*>(q + h * stride), f);
+  for (int h0 = 0; h0 < group; h0 += 4) {   // four rows at once: one after another they are four latencies
+    uint4 v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] += (W)(upper ? (f[i] < 0.f ? 0.f : f[i]) : (f[i] > 0.f ? 0.f : f[i]));
+    for (int u = 0; u < 4; ++u)
+      v[u] = h0 + u < group ? *reinterpret_cast<const uint4*>(q + (h0 + u) * stride) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float f[8];
+      to_f32x8(T{}, v[u], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] += (W)(upper ? (f[i] < 0.f ? 0.f : f[i]) : (f[i] > 0.f ? 0.f : f[i]));
+    }
   }
 }
 
@@ -179,6 +185,55 @@ constexpr int kBatch = 32;   // block ids that a warp holds
 constexpr int kStep = 4;     // pages of a lane's step
 constexpr int kRing = 3;     // steps in the copies' ring
 constexpr int ring_bytes(int threads) { return kRing * kStep * 16 * threads; }
+
+// One step's scores of a warp: v holds 16 bytes of each of kStep pages. Returns the lane's
+// page number within the step (of the sub-warp's kStep pages) in `at` and its score in s[0];
+// lanes with (lane & mask) == 0 hold one page each.
+template <typename T, int LP>
+__device__ __forceinline__ float step_scores(const uint4 (&v)[kStep], const float (&w)[8], int lane, uint32_t& largest,
+                                             int& at, int& mask) {
+  float s[kStep];
+#pragma unroll
+  for (int u = 0; u < kStep; ++u) {
+    float f[8];
+    to_f32x8(T{}, v[u], f);
+    float2 a = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a = fma2(make_float2(f[2 * i], f[2 * i + 1]), make_float2(w[2 * i], w[2 * i + 1]), a);
+    s[u] = a.x + a.y;
+    largest = max_abs2(T{}, max_abs2(T{}, max_abs2(T{}, largest, v[u].x), v[u].y), max_abs2(T{}, v[u].z, v[u].w));
+  }
+  // sums over the LP lanes of a page: first steps that also halve the pages a lane holds
+  at = 0;
+  int o = LP / 2;
+#pragma unroll
+  for (int h = kStep / 2; h >= 1; h >>= 1, o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < h; ++i) {
+      const float give = lane & o ? s[i] : s[i + h], keep = lane & o ? s[i + h] : s[i];
+      s[i] = keep + __shfl_xor_sync(~0u, give, o);
+    }
+    at += lane & o ? h : 0;
+  }
+  mask = 2 * o - 1;                                  // lanes below: copies of the same page
+#pragma unroll
+  for (; o; o >>= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
+  return s[0];
+}
+
+// Error of f32 scores: a term passes at most G - 1 roundings of 2^-24 in its weight (of
+// terms of one sign), 5 in the lane and 5 between lanes, so (G + 9) 2^-24 sum |w b|
+// <= (G + 9) 2^-24 sum_lanes largest * size (size: the lane's sum of |w|); 1.125 times
+// (G + 11) covers the roundings of the bound itself.
+template <typename T>
+__device__ __forceinline__ float score_error(uint32_t largest, float size, int group) {
+  float f[8];
+  to_f32x8(T{}, make_uint4(largest, 0, 0, 0), f);
+  float err = fmaxf(fabsf(f[0]), fabsf(f[1])) * size;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) err += __shfl_xor_sync(~0u, err, o);   // D = 64: both halves, an upper bound
+  return err * (1.125f / (1 << 24) * (group + 11));
+}
 
 // Keys of the f32 scores of the competing pages i0 .. i1 - 1 of a (sequence, KV head), by one
 // warp of a CTA of kThr threads, to keys[i]; returns the scores' error, and the smallest and
@@ -236,76 +291,83 @@ __device__ float score_pages(const SelectPagesParams& p, int b, int hk, int i0, 
   k_lo = ~0u;
   k_hi = 0;
   uint32_t largest = 0;                            // largest |bound| of this lane's channels, as a pair
-      for (int j = 0; j < steps; ++j) {
+  for (int j = 0; j < steps; ++j) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
     if (j + kRing - 1 < steps) issue(j + kRing - 1);   // into the slots of step j - 1
     asm volatile("cp.async.commit_group;" ::: "memory");
-    float s[kStep];
+    uint4 v[kStep];
 #pragma unroll
-    for (int u = 0; u < kStep; ++u) {
-      const uint4 v = *reinterpret_cast<const uint4*>(ring + ((j % kRing * kStep + u) * kThr + tid) * 16);
-      float f[8];
-      to_f32x8(T{}, v, f);
-      float2 a = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a = fma2(make_float2(f[2 * i], f[2 * i + 1]), make_float2(w[2 * i], w[2 * i + 1]), a);
-      s[u] = a.x + a.y;
-      largest = max_abs2(T{}, max_abs2(T{}, max_abs2(T{}, largest, v.x), v.y), max_abs2(T{}, v.z, v.w));
-    }
-    // sums over the LP lanes of a page: first steps that also halve the pages a lane holds
-    int at = j * kPer + sub * kStep, o = LP / 2;
-#pragma unroll
-    for (int h = kStep / 2; h >= 1; h >>= 1, o >>= 1) {
-#pragma unroll
-      for (int i = 0; i < h; ++i) {
-        const float give = lane & o ? s[i] : s[i + h], keep = lane & o ? s[i + h] : s[i];
-        s[i] = keep + __shfl_xor_sync(~0u, give, o);
-      }
-      at += lane & o ? h : 0;
-    }
-    const int last = o;                            // lanes below: copies of the same page
-#pragma unroll
-    for (; o; o >>= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
-    if ((lane & (2 * last - 1)) == 0 && i0 + at < i1) {
-      const uint32_t k = order_key(s[0]);
-      keys[i0 + at] = k;
+    for (int u = 0; u < kStep; ++u)
+      v[u] = *reinterpret_cast<const uint4*>(ring + ((j % kRing * kStep + u) * kThr + tid) * 16);
+    int at, mask;
+    const float s = step_scores<T, LP>(v, w, lane, largest, at, mask);
+    at += i0 + j * kPer + sub * kStep;
+    if ((lane & mask) == 0 && at < i1) {
+      const uint32_t k = order_key(s);
+      keys[at] = k;
       k_lo = min(k_lo, k);
       k_hi = max(k_hi, k);
     }
   }
-  // Error of these scores: a term passes at most G - 1 roundings of 2^-24 in its weight
-  // (of terms of one sign), 5 in the lane and 5 between lanes, so (G + 9) 2^-24
-  // sum |w b| <= (G + 9) 2^-24 sum_lanes largest * size; 1.125 times (G + 11) covers the
-  // roundings of the bound itself.
-  float err;
-  {
-    float f[8];
-    to_f32x8(T{}, make_uint4(largest, 0, 0, 0), f);
-    err = fmaxf(fabsf(f[0]), fabsf(f[1])) * size;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) err += __shfl_xor_sync(~0u, err, o);   // D = 64: both halves, an upper bound
-    err *= 1.125f / (1 << 24) * (p.group + 11);
-  }
+  const float err = score_error<T>(largest, size, p.group);
   k_lo = __reduce_min_sync(~0u, k_lo);
   k_hi = __reduce_max_sync(~0u, k_hi);
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   return err;
 }
 
+// Bulk copy of `bytes` (a multiple of 16, both addresses on 16 bytes) counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// The scores of a batch. A CTA takes the same pages of up to eight neighbouring KV heads (a
+// consumer warp per head; fewer heads: the warps share a stage's pages), so that a page's
+// bounds come in one piece: a producer warp brings pages as bulk copies into a ring of
+// stages. 64 sequences to 32768 tokens, 8 heads: 52.7 us, 5.4 TB/s, of which some 8 us pass
+// before the first page is scored. (512-byte pieces, a warp's own head copied by its lanes:
+// 56 us, whatever the depth and the occupancy; the queries' rows read one after another
+// instead of four at once: 57.)
+constexpr int kScoreThreads = kThreads + 32;
+constexpr int kScoreStages = 6;
+constexpr int kStageBytes = 16 * 1024;
+
+struct ScoreCtl {
+  uint64_t full[kScoreStages], empty[kScoreStages];
+  int abort_flag;
+};
+constexpr int kScoreSmem = kScoreStages * kStageBytes + (int)sizeof(ScoreCtl);
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesParams p) {
-  extern __shared__ __align__(16) uint8_t ring[];
+__global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPagesParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int LP = 2 * D / 8;                      // lanes of one page's bounds
+  constexpr int kPer = kStep * (32 / LP);            // pages of a warp's step
+  constexpr int kRowBytes = 4 * D;                   // bounds of one page and head
+  ScoreCtl* ctl = reinterpret_cast<ScoreCtl*>(smem + kScoreStages * kStageBytes);
+  volatile int* abort_flag = &ctl->abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // pick_kernel waits for all of this one
-  // The warps of a CTA take the same pages of up to eight KV heads, whose bounds lie side by
-  // side: 4 KB of a page are read together where a warp alone reads 512 bytes.
   const int abreast = min(p.num_kv_heads, kWarps), groups = (p.num_kv_heads + abreast - 1) / abreast;
-  const int parts = kWarps / abreast;                // shares of one CTA
-  if (warp >= parts * abreast) return;
+  const int parts = p.parts;                         // warps of one head
+  const int span = parts * kPer;                     // pages of a stage: 4 .. 32, a power of two
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kScoreStages; ++s) {
+      mbar_init(&ctl->full[s], 1);
+      mbar_init(&ctl->empty[s], parts * abreast);
+    }
+    ctl->abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  const bool producer = warp == kWarps;
+  if (!producer && warp >= parts * abreast) return;
   const auto count = [&](int b) { return (competing(p, pages_of(p, b)) + kRun - 1) / kRun * groups; };
   FlatItems<decltype(count)> all(count, p.n, lane);
-  const int shares = min((int)gridDim.x * parts, all.total);
-  const int share = blockIdx.x + warp / abreast * gridDim.x;
+  const int shares = min((int)gridDim.x, all.total), share = blockIdx.x;
   if (share >= shares) return;
   const int g1 = share_begin(all.total, share + 1, shares);
   int g = share_begin(all.total, share, shares);
@@ -313,17 +375,104 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
   all.place(g, b, first);
   int N = competing(p, pages_of(p, b)), runs = (N + kRun - 1) / kRun;
   int group = (g - first) / runs, run = (g - first) % runs;
+  const bool side_by_side = p.b_s1 == 2 * D;
+  const int e = lane % LP, sub = lane / LP;
+  const int d = (e * 8) % D;
+  int stage = 0, phase = 0, issued = 0;              // of the ring, through all segments
 
   while (g < g1) {
-    // the share's runs of this (sequence, KV head)
+    // the share's runs of this (sequence, group of KV heads)
     const int here = min(runs - run, g1 - g);
-    const int hk = min(group * abreast + warp % abreast, p.num_kv_heads - 1);   // the last group: the last head again
     const int i0 = run * kRun, i1 = min(i0 + here * kRun, N);   // competing pages i0 .. i1 - 1
-    uint32_t k_lo, k_hi;
-    const float err = score_pages<T, D, kThreads>(p, b, hk, i0, i1, ring,
-                                                  p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride, k_lo, k_hi);
-    uint4* about = p.runs + ((int64_t)b * p.num_kv_heads + hk) * p.run_stride + run;
-    for (int r = lane; r < here; r += 32) about[r] = make_uint4(__float_as_uint(err), k_lo, k_hi, 0);
+    const int head0 = group * abreast, heads = min(abreast, p.num_kv_heads - head0);
+    const int steps = (i1 - i0 + span - 1) / span;
+    if (producer) {
+      const int32_t* bt = p.block_table + b * p.bt_s0 + (int64_t)p.sinks * p.bt_s1;
+      const T* bounds = reinterpret_cast<const T*>(p.bounds) + (int64_t)head0 * p.b_s1;
+      auto blocks_from = [&](int i) {   // lane l: the block of competing page i + l
+        int blk = bt[(int64_t)min(i + lane, i1 - 1) * p.bt_s1];
+        if ((unsigned)blk >= (unsigned)p.num_blocks) {
+          record_status(p.status, STARKV_EBOUNDS);
+          blk = 0;
+        }
+        return blk;
+      };
+      int cur = 0, nxt = blocks_from(i0);
+      for (int j = 0; j < steps; ++j) {
+        const int at = j * span;                     // first page of the stage, from i0
+        if (at % kBatch == 0) {
+          cur = nxt;
+          nxt = blocks_from(i0 + at + kBatch);
+        }
+        const int blk = __shfl_sync(~0u, cur, (at + lane) % kBatch);
+        const int pages = min(span, i1 - i0 - at);
+        bool ok = mbar_wait(&ctl->empty[stage], phase ^ 1, abort_flag, p.status);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&ctl->full[stage], pages * heads * kRowBytes);
+        __syncwarp();
+        ++issued;
+        if (lane < pages) {
+          uint8_t* dst = smem + stage * kStageBytes + lane * abreast * kRowBytes;
+          const T* src = bounds + (int64_t)blk * p.b_s0;
+          if (side_by_side) {
+            bulk_load(dst, src, heads * kRowBytes, &ctl->full[stage]);
+          } else {
+            for (int h = 0; h < heads; ++h)
+              bulk_load(dst + h * kRowBytes, src + h * p.b_s1, kRowBytes, &ctl->full[stage]);
+          }
+        }
+        if (++stage == kScoreStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    } else {
+      const int h = warp % abreast, part = warp / abreast;
+      const int hk = min(head0 + h, p.num_kv_heads - 1);
+      float w[8];
+      query_side(reinterpret_cast<const T*>(p.q) + b * p.q_s0 + (int64_t)(hk * p.group) * p.q_s1 + d, p.q_s1, p.group,
+                 e * 8 >= D, w);
+      float size = 0.f;                              // sum of |w| of this lane's channels
+#pragma unroll
+      for (int i = 0; i < 8; ++i) size += fabsf(w[i]);
+      uint32_t k_lo = ~0u, k_hi = 0, largest = 0;    // largest |bound| of this lane's channels, as a pair
+      uint32_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride + i0;
+      for (int j = 0; j < steps; ++j) {
+        if (!__all_sync(~0u, mbar_wait(&ctl->full[stage], phase, abort_flag, p.status))) break;
+        const int first_page = part * kPer + sub * kStep;   // of the stage
+        const int left = i1 - i0 - j * span;
+        const uint8_t* src = smem + stage * kStageBytes + (first_page * abreast + h) * kRowBytes + e * 16;
+        uint4 v[kStep];
+#pragma unroll
+        for (int u = 0; u < kStep; ++u)              // a page past the end, a head past the last: nothing was copied
+          v[u] = first_page + u < left && h < heads ? *reinterpret_cast<const uint4*>(src + u * abreast * kRowBytes)
+                                                    : make_uint4(0, 0, 0, 0);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->empty[stage]);
+        if (++stage == kScoreStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+        int at, mask;
+        const float s = step_scores<T, LP>(v, w, lane, largest, at, mask);
+        at += first_page;
+        if ((lane & mask) == 0 && at < left && h < heads) {
+          const uint32_t k = order_key(s);
+          keys[j * span + at] = k;
+          k_lo = min(k_lo, k);
+          k_hi = max(k_hi, k);
+        }
+      }
+      const float err = score_error<T>(largest, size, p.group);
+      k_lo = __reduce_min_sync(~0u, k_lo);
+      k_hi = __reduce_max_sync(~0u, k_hi);
+      // an entry per run and warp of the head
+      uint4* about = p.runs + (((int64_t)b * p.num_kv_heads + hk) * p.run_stride + run) * parts + part;
+      if (h < heads)
+        for (int r = lane; r < here; r += 32) about[r * parts] = make_uint4(__float_as_uint(err), k_lo, k_hi, 0);
+    }
+    if (*abort_flag) break;
     g += here;
     run = 0;
     if (g < g1 && ++group == groups) {
@@ -334,12 +483,17 @@ __global__ void __launch_bounds__(kThreads, 3) score_kernel(const SelectPagesPar
       runs = (N + kRun - 1) / kRun;
     }
   }
+  if (producer && *abort_flag) {   // no copy may land in shared memory that is no longer this CTA's
+    for (int k = max(0, issued - kScoreStages); k < issued; ++k)
+      for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(&ctl->full[k % kScoreStages], (k / kScoreStages) & 1); ++i) {
+      }
+  }
 }
 
 constexpr int kPickWarpsMost = 32;
 constexpr int kAhead = 4;         // keys in flight per thread
 constexpr int kPickCache = 8192;  // keys that are copied to shared memory
-constexpr int kFusedPages = 512, kFusedThreads = 512;   // pages that pick_kernel scores itself
+constexpr int kFusedFew = 384, kFusedPages = 512, kFusedThreads = 512;   // pages that pick_kernel scores itself
 
 constexpr int kBins = 2048;
 constexpr int kNear = 256;        // pages next to the border that are scored again one by one
@@ -523,8 +677,8 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
   } else {
     asm volatile("griddepcontrol.wait;" ::: "memory");   // the scores are written
     if (N == 0) return;
-    const uint4* runs = p.runs + (int64_t)unit * p.run_stride;
-    const int n_runs = (N + kRun - 1) / kRun;
+    const uint4* runs = p.runs + (int64_t)unit * p.run_stride * p.parts;
+    const int n_runs = (N + kRun - 1) / kRun * p.parts;
     uint4 about = runs[min(tid, n_runs - 1)];
     if (N <= kCache) {
       for (int i = tid; i < N; i += 2 * kAhead * kThr) {
@@ -775,9 +929,10 @@ template <typename T, int D>
 int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
   const int64_t units = (int64_t)p.n * p.num_kv_heads;
   p.run_stride = (p.key_stride + kRun - 1) / kRun;
+  p.parts = std::min(kWarps / std::min(p.num_kv_heads, kWarps), 32 / (kStep * (128 / D)));
   if (units * p.run_stride > 0x7fffffff) return STARKV_EINVAL;   // 32-bit run numbers
   p.runs = reinterpret_cast<uint4*>(p.scratch);
-  p.exact = reinterpret_cast<uint64_t*>(p.runs + units * p.run_stride);
+  p.exact = reinterpret_cast<uint64_t*>(p.runs + units * p.run_stride * p.parts);
   p.keys = reinterpret_cast<uint32_t*>(p.exact + units * p.key_stride);
   void* args[] = {&p};
   cudaLaunchConfig_t cfg = {};
@@ -787,10 +942,11 @@ int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
   cfg.gridDim = dim3((unsigned)units);
   cfg.stream = stream;
   cfg.attrs = attr;
-  // One kernel where a CTA per unit, one to an SM, is enough for the reads (8 units of 256 /
-  // 512 / 1024 pages: 13.6 / 16 / 20.6 us against 14.2 / 14.3 / 14.4 in two, 32 units of 281
-  // small pages 15.1 against 17.7; and a launch less, 4 us of the host's time).
-  if (units <= num_sms && p.key_stride <= kFusedPages) {
+  // One kernel where a CTA per unit, one to an SM, is enough for the reads. Its time grows
+  // with the pages of a unit, that of two kernels with all pages: 8 units of 128 / 375 / 512
+  // pages 12.6 / 13.3 / 16.5 us against 11.9 / 11.6 / 12.6 in two; 128 units of 256 / 512
+  // pages 13.6 / 15.7 against 16.7 / 19.2. The launch less is 4 us of the host's time.
+  if (units <= num_sms && p.key_stride <= (units < 64 ? kFusedFew : kFusedPages)) {
     const void* fn = (const void*)pick_kernel<T, D, kFusedThreads, true>;
     if (const int st = allow_smem(fn, ring_bytes(kFusedThreads))) return st;
     cfg.blockDim = dim3(kFusedThreads);
@@ -799,9 +955,9 @@ int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
   }
   if (p.key_stride > p.top) {   // else no sequence has pages to choose from
     const void* fn = (const void*)score_kernel<T, D>;
-    if (const int st = allow_smem(fn, ring_bytes(kThreads))) return st;
-    const int64_t grid = std::min<int64_t>(3 * num_sms, units * p.run_stride);
-    if (cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), args, ring_bytes(kThreads), stream) != cudaSuccess)
+    if (const int st = allow_smem(fn, kScoreSmem)) return st;
+    const int64_t grid = std::min<int64_t>(2 * num_sms, units * p.run_stride);
+    if (cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kScoreThreads), args, kScoreSmem, stream) != cudaSuccess)
       return STARKV_ECUDA;
   }
   const bool few = units <= num_sms && p.key_stride > 1024;
@@ -826,7 +982,7 @@ int launch_bounds_typed(PageBoundsParams p, cudaStream_t stream) {
 }  // namespace
 
 size_t select_scratch_bytes(int64_t units, int64_t pages) {
-  return (size_t)units * (pages * 12 + (pages + kRun - 1) / kRun * 16);
+  return (size_t)units * (pages * 12 + (pages + kRun - 1) / kRun * 16 * kWarps);   // at most kWarps entries a run
 }
 
 int launch_page_bounds(const PageBoundsParams& p, int dtype, int head_dim, cudaStream_t stream) {

@@ -177,7 +177,7 @@ struct SelectPagesParams {
   void* scratch; int64_t key_stride;                 // pages of the longest sequence
   // set by the launch, in `scratch`: per run of pages {error, smallest key, largest key};
   // order keys of the 32-bit scores and, where they do not decide, of the 64-bit ones
-  uint4* runs; int64_t run_stride;                   // [n, KV heads, run_stride]
+  uint4* runs; int64_t run_stride; int parts;        // [n, KV heads, run_stride, parts]
   uint32_t* keys; uint64_t* exact;                   // [n, KV heads, key_stride]
   int32_t* pages; int64_t pg_s0, pg_s1;              // [n, KV heads, top]
   int32_t* status;
