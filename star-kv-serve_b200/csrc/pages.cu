@@ -150,11 +150,15 @@ __device__ __forceinline__ uint32_t max_abs2(__half, uint32_t a, uint32_t b) {
   return d;
 }
 
-// up (upper) or down of channels d .. d + 7 of a KV head's queries
+// up (upper) or down of channels d .. d + 7 of a KV head's queries. In few instructions,
+// as pick_kernel's steps are: each kernel of a selection runs its code once per CTA, so the
+// time of its straight parts is that of fetching them (f32 compares in place of the packed
+// max: 7000 cycles instead of 1000 at the start of score_kernel).
 template <typename T, typename W>
 __device__ __forceinline__ void query_side(const T* q, int64_t stride, int group, bool upper, W (&w)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 0;
+  const uint32_t flip = upper ? 0u : 0x80008000u;
   for (int h0 = 0; h0 < group; h0 += 4) {   // four rows at once: one after another they are four latencies
     uint4 v[4];
 #pragma unroll
@@ -162,10 +166,16 @@ __device__ __forceinline__ void query_side(const T* q, int64_t stride, int group
       v[u] = h0 + u < group ? *reinterpret_cast<const uint4*>(q + (h0 + u) * stride) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      float f[8];
-      to_f32x8(T{}, v[u], f);
+      uint4 r = v[u];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] += (W)(upper ? (f[i] < 0.f ? 0.f : f[i]) : (f[i] > 0.f ? 0.f : f[i]));
+      for (int i = 0; i < 4; ++i) {
+        uint32_t& x = (&r.x)[i];
+        x = max2(T{}, x ^ flip, 0u) ^ flip;              // -max(-x, 0) = min(x, 0); a NaN stays one
+      }
+      float f[8];
+      to_f32x8(T{}, r, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] += (W)f[i];
     }
   }
 }
@@ -327,10 +337,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, int bytes,
 // The scores of a batch. A CTA takes the same pages of up to eight neighbouring KV heads (a
 // consumer warp per head; fewer heads: the warps share a stage's pages), so that a page's
 // bounds come in one piece: a producer warp brings pages as bulk copies into a ring of
-// stages. 64 sequences to 32768 tokens, 8 heads: 52.7 us, 5.4 TB/s, of which some 8 us pass
-// before the first page is scored. (512-byte pieces, a warp's own head copied by its lanes:
-// 56 us, whatever the depth and the occupancy; the queries' rows read one after another
-// instead of four at once: 57.)
+// stages. 64 sequences to 32768 tokens, 8 heads: 52 us, 5.4 TB/s, of which 4.7 us pass before
+// the first page is scored. (512-byte pieces, a warp's own head copied by its lanes:
+// 56 us, whatever the depth and the occupancy.)
 constexpr int kScoreThreads = kThreads + 32;
 constexpr int kScoreStages = 6;
 constexpr int kStageBytes = 16 * 1024;
@@ -580,7 +589,7 @@ __device__ void write_selected(int N, PickShared& sh, const Cls& cls, int rest, 
   int gt0 = 0, eq0 = 0;                              // of the rounds before
   for (int r0 = 0; r0 < N; r0 += 32 * 256) {
     const int words = min(256, (N - r0 + 31) / 32);
-#pragma unroll 4
+#pragma unroll 1
     for (int w = warp; w < words; w += kThr / 32) {
       const int i = r0 + w * 32 + lane;
       const int c = i < N ? cls(i) : 0;
@@ -606,25 +615,17 @@ __device__ void write_selected(int N, PickShared& sh, const Cls& cls, int rest, 
       sh.eq[warp] = eq;
     }
     __syncthreads();
-    int gt_all = 0, eq_all = 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      if (w < warp) {
-        gt += sh.gt[w];
-        eq += sh.eq[w];
-      }
-      gt_all += sh.gt[w];
-      eq_all += sh.eq[w];
-    }
-    gt += gt0 - __popc(g);                           // before this thread's pages
-    eq += eq0 - __popc(e);
+    const int gt_w = lane < 8 ? sh.gt[lane] : 0, eq_w = lane < 8 ? sh.eq[lane] : 0;
+    // before this thread's pages
+    gt += gt0 - __popc(g) + __reduce_add_sync(~0u, lane < warp ? gt_w : 0);
+    eq += eq0 - __popc(e) + __reduce_add_sync(~0u, lane < warp ? eq_w : 0);
     for (uint32_t m = g | e; m; m &= m - 1) {
       const uint32_t bit = m & -m;
       if (g & bit) out[gt++ + min(eq, rest)] = base + r0 + tid * 32 + __ffs(bit) - 1;
       else if (eq++ < rest) out[gt + eq - 1] = base + r0 + tid * 32 + __ffs(bit) - 1;
     }
-    gt0 += gt_all;
-    eq0 += eq_all;
+    gt0 += __reduce_add_sync(~0u, gt_w);
+    eq0 += __reduce_add_sync(~0u, eq_w);
     __syncthreads();
   }
 }
@@ -713,11 +714,11 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
     sh.off = 0;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThr / 32; ++w) {
-    e_bits = max(e_bits, (uint32_t)sh.lo[w]);
-    k_lo = min(k_lo, (uint32_t)(sh.lo[w] >> 32));
-    k_hi = max(k_hi, (uint32_t)sh.hi[w]);
+  {
+    const int w = min(lane, kThr / 32 - 1);
+    e_bits = __reduce_max_sync(~0u, (uint32_t)sh.lo[w]);
+    k_lo = __reduce_min_sync(~0u, (uint32_t)(sh.lo[w] >> 32));
+    k_hi = __reduce_max_sync(~0u, (uint32_t)sh.hi[w]);
   }
   const int need = p.top - p.sinks - p.recent;       // < N
   const float err = __uint_as_float(e_bits), reach = 2.01f * err;
@@ -792,7 +793,7 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
     }
     if (lane == 31 && warp < 8) sh.scan[warp] = incl;
     __syncthreads();
-    for (int w = 0; w < min(warp, 8); ++w) incl += sh.scan[w];
+    incl += __reduce_add_sync(~0u, lane < min(warp, 8) ? sh.scan[lane] : 0u);
     if (warp < 8 && incl >= (uint32_t)need && incl - mine < (uint32_t)need) {
       const uint32_t c[8] = {x.w, x.z, x.y, x.x, y.w, y.z, y.y, y.x};
       uint32_t sum = incl - mine;
