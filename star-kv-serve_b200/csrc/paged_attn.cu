@@ -320,17 +320,15 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
     // valid bits of the kStages - 1 = 2 subtiles in flight
     uint32_t va = 0, vb = 0;
     static_assert(kStages == 3, "two subtiles in flight");
-    if (subs > 0) va = issue(0);
-    cp_commit();
-    if (subs > 1) vb = issue(1);
-    cp_commit();
-    for (int i = 0; i < subs; ++i) {
+    // (one place that issues: the kernel's first pass over its code is fetched from memory)
+    for (int i = -2; i < subs; ++i) {
       cp_wait<kStages - 2>();
       __syncwarp();   // every lane's copies of subtile i are in; every lane is done with subtile i - 1
       const uint32_t valid = va;
       va = vb;
       if (i + 2 < subs) vb = issue(i + 2);
       cp_commit();
+      if (i < 0) continue;
       const uint32_t kt = ring + (i % kStages) * R::stage_bytes, vt = kt + R::op_bytes;
       const int mi = lane >> 3, rr = lane & 7;
       // ---- S = Q K^T, 16 tokens ----
