@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPag
 constexpr int kPickWarpsMost = 32;
 constexpr int kAhead = 4;         // keys in flight per thread
 constexpr int kPickCache = 8192;  // keys that are copied to shared memory
-constexpr int kFusedFew = 384, kFusedPages = 512, kFusedThreads = 512;   // pages that pick_kernel scores itself
+constexpr int kFusedPages = 512, kFusedThreads = 512;   // pages that pick_kernel scores itself
 
 constexpr int kBins = 2048;
 constexpr int kNear = 256;        // pages next to the border that are scored again one by one
@@ -945,9 +945,9 @@ int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
   cfg.attrs = attr;
   // One kernel where a CTA per unit, one to an SM, is enough for the reads. Its time grows
   // with the pages of a unit, that of two kernels with all pages: 8 units of 128 / 375 / 512
-  // pages 12.6 / 13.3 / 16.5 us against 11.9 / 11.6 / 12.6 in two; 128 units of 256 / 512
-  // pages 13.6 / 15.7 against 16.7 / 19.2. The launch less is 4 us of the host's time.
-  if (units <= num_sms && p.key_stride <= (units < 64 ? kFusedFew : kFusedPages)) {
+  // / 1024 pages 7.2 / 8.9 / 12.0 / 15.9 us against 9.5 / 9.1 / 10.3 / 10.0 in two; 128 units
+  // of 256 / 512 pages 9.3 / 11.4 against 12.2 / 14.4. The launch less is 4 us of the host's.
+  if (units <= num_sms && p.key_stride <= kFusedPages) {
     const void* fn = (const void*)pick_kernel<T, D, kFusedThreads, true>;
     if (const int st = allow_smem(fn, ring_bytes(kFusedThreads))) return st;
     cfg.blockDim = dim3(kFusedThreads);
