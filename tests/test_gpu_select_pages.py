@@ -301,3 +301,18 @@ def test_given_outputs_strided_bounds_and_empty_batches():
     update_page_bounds(k, bounds, bt[:0], sl[:0], 900)
     update_page_bounds(k, bounds, bt, sl, 900, max_new=0)
     assert torch.equal(wide, before)
+
+
+@pytest.mark.parametrize("Hkv,D", [(1, 128), (3, 64), (8, 128), (11, 64), (20, 128)])
+@pytest.mark.parametrize("apart", [False, True])
+def test_long_units_of_neighbouring_heads(Hkv, D, apart):
+    """More pages than one kernel takes; the bounds of a page's heads in one piece, or apart."""
+    from starkv_b200.kernels.paged_attention import empty_bounds, select_pages, update_page_bounds
+    import test_gpu_paged_attention as A
+    q, k, v, bt, sl = A.make([8999, 20, 9600], 2 * Hkv, Hkv, D=D, seed=70 + Hkv)
+    bounds = empty_bounds(k)
+    if apart:
+        bounds = torch.full((k.shape[0], Hkv, 4, D), 7.0, dtype=k.dtype, device=k.device)[:, :, 1:3]
+    update_page_bounds(k, bounds, bt, sl, 9600, max_new=9600)
+    got = select_pages(q, bounds, bt, sl, 9600, 16, 37)
+    assert torch.equal(got.cpu(), expected(q, bounds, bt, sl.tolist(), 16, 37, 1, 1))
