@@ -22,18 +22,7 @@ DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
 EPS = 1e-6
 
 
-_kernels = None
-
-
 def kernels():
-    """The framework's modules, imported once as a program does at its start."""
-    global _kernels
-    if _kernels is None:
-        _kernels = _import_kernels()
-    return _kernels
-
-
-def _import_kernels():
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "star-kv-serve_b200")
     if path not in sys.path:
         sys.path.insert(0, path)
