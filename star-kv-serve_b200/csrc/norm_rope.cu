@@ -69,7 +69,8 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 // 8 / D heads a step: token, kind, table row and cache slot are the warp's, so a row costs
 // little more than its own arithmetic (8191 tokens of 48 heads, f16: 41 us, 5.0 TB/s; with
 // token and heads chosen per group of lanes 193 instructions a warp and step, and 51 us).
-template <typename T, int D, int kSteps>
+// kPart: the table is narrower than a head (asked in the loop of every call: 45 us).
+template <typename T, int D, int kSteps, bool kPart>
 __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeParams p, unsigned q_chunks,
                                                              unsigned k_chunks, unsigned chunks, unsigned items) {
   constexpr int kLanes = D / 8, G = 32 / kLanes;
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeParam
 
   // out_lo = inv * (x_lo a + x_hi b), out_hi = inv * (x_hi c + x_lo d): the weight is in a .. d already
   float4 a = make_float4(1.f, 1.f, 1.f, 1.f), b = make_float4(0.f, 0.f, 0.f, 0.f), c = a, d = b;
-  if (j < pairs) {
+  if (!kPart || j < pairs) {
     int64_t pos = load_slot(p.positions, t, p.pos_dtype);
     if (pos < 0 || pos >= p.table_rows) {
       record_status(p.status, STARKV_EBOUNDS);
@@ -198,8 +199,14 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeParam
     for (int u = 0; u < kAhead; ++u) {
       const float2 l0 = unpack(T{}, raw[u][0].x), l1 = unpack(T{}, raw[u][0].y);
       const float2 h0v = unpack(T{}, raw[u][1].x), h1v = unpack(T{}, raw[u][1].y);
-      float2 x0 = fma2(h0v, b0, mul2(l0, a0)), x1 = fma2(h1v, b1, mul2(l1, a1));
-      float2 y0 = fma2(l0, d0, mul2(h0v, c0)), y1 = fma2(l1, d1, mul2(h1v, c1));
+      float2 x0 = mul2(l0, a0), x1 = mul2(l1, a1), y0 = mul2(h0v, c0), y1 = mul2(h1v, c1);
+      // not by zeros in b and d: behind the rotated width an infinity stays its own channel's
+      if (!kPart || j < pairs) {
+        x0 = fma2(h0v, b0, x0);
+        x1 = fma2(h1v, b1, x1);
+        y0 = fma2(l0, d0, y0);
+        y1 = fma2(l1, d1, y1);
+      }
       if (w) {
         const float2 iv = make_float2(inv[u], inv[u]);
         x0 = mul2(iv, x0);
@@ -232,8 +239,10 @@ int launch_steps(const NormRopeParams& p, cudaStream_t stream) {
   if ((int64_t)p.n * chunks > 0x7fffffff) return STARKV_EINVAL;
   unsigned items = (unsigned)p.n * chunks;
   void* args[] = {const_cast<NormRopeParams*>(&p), &qc, &kc, &chunks, &items};
-  return cudaLaunchKernel((const void*)norm_rope_kernel<T, D, kSteps>, dim3((items + kThreads / 32 - 1) / (kThreads / 32)),
-                          dim3(kThreads), args, 0, stream) == cudaSuccess
+  const void* fn = p.rot < D ? (const void*)norm_rope_kernel<T, D, kSteps, true>
+                             : (const void*)norm_rope_kernel<T, D, kSteps, false>;
+  return cudaLaunchKernel(fn, dim3((items + kThreads / 32 - 1) / (kThreads / 32)), dim3(kThreads), args, 0, stream) ==
+                 cudaSuccess
              ? STARKV_OK
              : STARKV_ECUDA;
 }
