@@ -16,7 +16,8 @@
 // is split; 32-bit sums put about one of a thousand selections on the other side). 64-bit
 // conversions run at an eighth of the rate that the reads need, so score_kernel sums in
 // f32 and also bounds the error, and pick_kernel sums again in 64 bits only the pages
-// that lie within the error of the border, mostly none.
+// that lie within the error of the border, mostly none. The bound covers products too
+// small for f32; sums too large for it have no bound, and pick_kernel sums all pages again.
 //
 // score_kernel takes the batch's pages in runs of 16, an equal number of runs per CTA
 // whatever the mix of lengths, and writes order-preserving keys. pick_kernel takes a CTA
@@ -234,15 +235,20 @@ __device__ __forceinline__ float step_scores(const uint4 (&v)[kStep], const floa
 // Error of f32 scores: a term passes at most G - 1 roundings of 2^-24 in its weight (of
 // terms of one sign), 5 in the lane and 5 between lanes, so (G + 9) 2^-24 sum |w b|
 // <= (G + 9) 2^-24 sum_lanes largest * size (size: the lane's sum of |w|); 1.125 times
-// (G + 11) covers the roundings of the bound itself.
+// (G + 11) covers the roundings of the bound itself. Below 2^-126 a product is off by up to
+// 2^-150 instead, 256 of them by 2^-142: 2^-120 times the factor is more. 0 only where every
+// term is one of zeros. INFINITY where a sum may have left f32's range (it is at most the
+// sum of |w b|) or a factor is not finite: then the scores say nothing, NaN ones neither.
 template <typename T>
 __device__ __forceinline__ float score_error(uint32_t largest, float size, int group) {
   float f[8];
   to_f32x8(T{}, make_uint4(largest, 0, 0, 0), f);
-  float err = fmaxf(fabsf(f[0]), fabsf(f[1])) * size;
+  const float most = fmaxf(fabsf(f[0]), fabsf(f[1]));
+  float err = most * size;
+  if (most > 0.f && size > 0.f) err += 0x1p-120f;
 #pragma unroll
   for (int o = 16; o; o >>= 1) err += __shfl_xor_sync(~0u, err, o);   // D = 64: both halves, an upper bound
-  return err * (1.125f / (1 << 24) * (group + 11));
+  return err < 1e38f ? err * (1.125f / (1 << 24) * (group + 11)) : INFINITY;   // a NaN too
 }
 
 // Keys of the f32 scores of the competing pages i0 .. i1 - 1 of a (sequence, KV head), by one
@@ -673,8 +679,7 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
     const int per = ((N + kThr / 32 - 1) / (kThr / 32) + 7) & ~7;
     if (warp * per < N)
       e_bits = __float_as_uint(score_pages<T, D, kThr>(p, b, hk, warp * per, min((warp + 1) * per, N), ring, cache, k_lo,
-                                                       k_hi)) &
-               0x7fffffffu;
+                                                       k_hi));
   } else {
     asm volatile("griddepcontrol.wait;" ::: "memory");   // the scores are written
     if (N == 0) return;
@@ -693,7 +698,7 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
       keys = cache;
     }
     for (int r = tid;;) {
-      e_bits = max(e_bits, about.x & 0x7fffffffu);   // >= 0 or NaN: ordered as integers
+      e_bits = max(e_bits, about.x);                 // >= 0: ordered as integers
       k_lo = min(k_lo, about.y);
       k_hi = max(k_hi, about.z);
       if ((r += kThr) >= n_runs) break;
@@ -861,7 +866,8 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
     in = min(in, (uint32_t)sh.lo[w]);
     off = max(off, (uint32_t)sh.hi[w]);
   }
-  const bool nan = in == ~0u;                        // the border lies among NaN scores: all the same
+  // the border lies among NaN scores: all the same, if the scores are to be believed
+  const bool nan = in == ~0u && reach < INFINITY;
   const float at = key_value(in);
   // sure: every selected score is further above every other than the error can move them
   if (err == 0.f || nan || (whole && at - key_value(off) > reach)) {
@@ -873,11 +879,14 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
   }
 
   // 64-bit scores of the pages within reach of the border; above it all are selected,
-  // below it none. Not a number of an error: every page but the NaN ones.
+  // below it none. No bound of the error: of every page, the keys of NaN scores among them.
   uint32_t near_lo = 0, near_hi = ~0u - 1;
   if (reach < INFINITY) {
     near_lo = max(order_key(at - reach), 1u) - 1;
     near_hi = min(order_key(at + reach), ~0u - 2) + 1;
+  } else {
+    for (int i = tid; i < N; i += kThr) keys[i] = min(keys[i], near_hi);
+    __syncthreads();
   }
   list_near(near_lo, near_hi);
   const int near = sh.near, open = need - sh.above;  // pages to be told apart, and how many of them are selected
