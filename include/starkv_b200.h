@@ -166,7 +166,7 @@ STARKV_API int starkv_paged_decode_q32_partial(const StarKVDecodeArgs* args, int
 /*
  * Self-test of the kernels' bounded pipeline waits (no counterpart in the
  * reference): one thread waits on a barrier that nothing completes. The wait gives
- * up after its poll limit (about a second) and records STARKV_ETIMEOUT in the
+ * up after its poll limit (16 s measured) and records STARKV_ETIMEOUT in the
  * device status word `status` (caller-zeroed int32), as every pipeline wait in
  * the decode kernels does instead of hanging.
  */
@@ -351,6 +351,16 @@ STARKV_API size_t starkv_select_pages_workspace_bytes(int32_t n, int32_t num_kv_
                                                       int32_t block_size, int32_t top);
 STARKV_API int starkv_select_pages(const StarKVSelectPagesArgs* args, void* workspace, size_t workspace_bytes,
                                    void* stream);
+
+/*
+ * Self-test of the selection's bounded waits: starkv_select_pages whose scoring kernel (more
+ * than 512 pages in the longest sequence, or more units than SMs) is never given its data.
+ * Its waits run out (16 s measured), STARKV_ETIMEOUT is recorded in args->status, and the
+ * lists of the sequences that have pages to choose from hold -1 throughout, as after any
+ * expired wait.
+ */
+STARKV_API int starkv_selftest_select_timeout(const StarKVSelectPagesArgs* args, void* workspace,
+                                              size_t workspace_bytes, void* stream);
 
 /*
  * starkv_select_pages, then starkv_paged_attention over the selected pages, the second

@@ -695,6 +695,18 @@ int starkv_select_pages(const StarKVSelectPagesArgs* a, void* workspace, size_t 
   return launch_select_pages(p, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream);
 }
 
+int starkv_selftest_select_timeout(const StarKVSelectPagesArgs* a, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  using namespace starkv;
+  SelectPagesParams p;
+  bool done;
+  if (const int st = select_pages_params(a, workspace, workspace_bytes, p, done); st || done) return st;
+  DeviceInfo dev;
+  if (const int st = device_info(dev)) return st;
+  p.stall = 1;
+  return launch_select_pages(p, a->dtype, a->head_dim, dev.sms, (cudaStream_t)stream);
+}
+
 int starkv_sparse_paged_attention(const StarKVPagedAttnArgs* a, const void* bounds, int64_t bounds_stride0,
                                   int64_t bounds_stride1, int32_t sinks, int32_t recent, void* workspace,
                                   size_t workspace_bytes, void* stream) {

@@ -192,6 +192,7 @@ __device__ __forceinline__ int competing(const SelectPagesParams& p, int pages) 
 }
 
 constexpr int kRun = 16;     // pages of a run
+constexpr uint32_t kGaveUp = ~0u;   // in the place of a run's error: a wait ran out, it has no scores
 constexpr int kBatch = 32;   // block ids that a warp holds
 constexpr int kStep = 4;     // pages of a lane's step
 constexpr int kRing = 3;     // steps in the copies' ring
@@ -394,6 +395,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPag
   const int e = lane % LP, sub = lane / LP;
   const int d = (e * 8) % D;
   int stage = 0, phase = 0, issued = 0;              // of the ring, through all segments
+  bool ok = true;                                    // no wait of this warp has run out
 
   while (g < g1) {
     // the share's runs of this (sequence, group of KV heads)
@@ -413,7 +415,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPag
         return blk;
       };
       int cur = 0, nxt = blocks_from(i0);
-      for (int j = 0; j < steps; ++j) {
+      for (int j = 0; j < steps && !p.stall; ++j) {
         const int at = j * span;                     // first page of the stage, from i0
         if (at % kBatch == 0) {
           cur = nxt;
@@ -421,8 +423,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPag
         }
         const int blk = __shfl_sync(~0u, cur, (at + lane) % kBatch);
         const int pages = min(span, i1 - i0 - at);
-        bool ok = mbar_wait(&ctl->empty[stage], phase ^ 1, abort_flag, p.status);
-        ok = __all_sync(~0u, ok);
+        ok = __all_sync(~0u, mbar_wait(&ctl->empty[stage], phase ^ 1, abort_flag, p.status));
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&ctl->full[stage], pages * heads * kRowBytes);
         __syncwarp();
@@ -453,8 +454,9 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPag
       for (int i = 0; i < 8; ++i) size += fabsf(w[i]);
       uint32_t k_lo = ~0u, k_hi = 0, largest = 0;    // largest |bound| of this lane's channels, as a pair
       uint32_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + hk) * p.key_stride + i0;
-      for (int j = 0; j < steps; ++j) {
-        if (!__all_sync(~0u, mbar_wait(&ctl->full[stage], phase, abort_flag, p.status))) break;
+      for (int j = 0; ok && j < steps; ++j) {        // after a wait that ran out no stage is what it should be
+        ok = __all_sync(~0u, mbar_wait(&ctl->full[stage], phase, abort_flag, p.status));
+        if (!ok) break;
         const int first_page = part * kPer + sub * kStep;   // of the stage
         const int left = i1 - i0 - j * span;
         const uint8_t* src = smem + stage * kStageBytes + (first_page * abreast + h) * kRowBytes + e * 16;
@@ -482,12 +484,12 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPag
       const float err = score_error<T>(largest, size, p.group);
       k_lo = __reduce_min_sync(~0u, k_lo);
       k_hi = __reduce_max_sync(~0u, k_hi);
-      // an entry per run and warp of the head
+      // an entry per run and warp of the head, on every path: pick_kernel reads all of them
       uint4* about = p.runs + (((int64_t)b * p.num_kv_heads + hk) * p.run_stride + run) * parts + part;
       if (h < heads)
-        for (int r = lane; r < here; r += 32) about[r * parts] = make_uint4(__float_as_uint(err), k_lo, k_hi, 0);
+        for (int r = lane; r < here; r += 32) about[r * parts] = make_uint4(ok ? __float_as_uint(err) : kGaveUp, k_lo, k_hi, 0);
     }
-    if (*abort_flag) break;
+    if (producer && !ok) break;
     g += here;
     run = 0;
     if (g < g1 && ++group == groups) {
@@ -498,7 +500,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPag
       runs = (N + kRun - 1) / kRun;
     }
   }
-  if (producer && *abort_flag) {   // no copy may land in shared memory that is no longer this CTA's
+  if (producer) {   // no copy may land in shared memory that is no longer this CTA's, whoever gave up
     for (int k = max(0, issued - kScoreStages); k < issued; ++k)
       for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(&ctl->full[k % kScoreStages], (k / kScoreStages) & 1); ++i) {
       }
@@ -724,6 +726,10 @@ __global__ void __launch_bounds__(kThr, 1024 / kThr) pick_kernel(const SelectPag
     e_bits = __reduce_max_sync(~0u, (uint32_t)sh.lo[w]);
     k_lo = __reduce_min_sync(~0u, (uint32_t)(sh.lo[w] >> 32));
     k_hi = __reduce_max_sync(~0u, (uint32_t)sh.hi[w]);
+  }
+  if (!kFused && e_bits == kGaveUp) {                // the same for the whole CTA: a list of no pages
+    for (int i = tid; i < p.top; i += kThr) out[i - p.sinks] = -1;
+    return;
   }
   const int need = p.top - p.sinks - p.recent;       // < N
   const float err = __uint_as_float(e_bits), reach = 2.01f * err;

@@ -181,6 +181,7 @@ struct SelectPagesParams {
   uint32_t* keys; uint64_t* exact;                   // [n, KV heads, key_stride]
   int32_t* pages; int64_t pg_s0, pg_s1;              // [n, KV heads, top]
   int32_t* status;
+  int stall;                                         // self-test: score_kernel's producer brings nothing
 };
 
 struct NormRopeParams {

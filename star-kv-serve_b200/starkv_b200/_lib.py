@@ -158,6 +158,7 @@ EXPORTS = {
     "starkv_page_bounds": (C.c_int, [C.c_char_p, p]),
     "starkv_select_pages_workspace_bytes": (C.c_size_t, [i32, i32, i32, i32, i32]),
     "starkv_select_pages": (C.c_int, [C.c_char_p, p, C.c_size_t, p]),
+    "starkv_selftest_select_timeout": (C.c_int, [C.c_char_p, p, C.c_size_t, p]),
     "starkv_sparse_paged_attention": (C.c_int, [C.c_char_p, p, i64, i64, i32, i32, p, C.c_size_t, p]),
     "starkv_norm_rope": (C.c_int, [C.c_char_p, p]),
     "starkv_cache_write_bf16": (C.c_int, [C.POINTER(CacheWriteArgs), p]),
