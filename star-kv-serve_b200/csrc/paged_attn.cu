@@ -131,6 +131,31 @@ constexpr float weight_bias() {
   return std::is_same<T, __half>::value ? 10.f : 0.f;
 }
 
+// (a, b) += (c, d)
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
+  asm("{.reg .b64 x, y; mov.b64 x, {%0, %1}; mov.b64 y, {%2, %3}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x;}"
+      : "+f"(a), "+f"(b) : "f"(c), "f"(d));
+}
+__device__ __forceinline__ bool finite4(float4 v) {
+  return fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY;
+}
+// An infinite V meets parts of its weight that are 0 or below it, and weights of shares that
+// have become 0: NaN. With weights > 0 the sum is that of the channel's infinities and NaN,
+// so where a result of a finite denominator is not finite those alone are added up:
+// `odd` takes what of v is not finite, and replaces what it has of acc.
+__device__ __forceinline__ void add_odd(float4& odd, float4 v) {
+  odd.x += fabsf(v.x) < INFINITY ? 0.f : v.x;
+  odd.y += fabsf(v.y) < INFINITY ? 0.f : v.y;
+  odd.z += fabsf(v.z) < INFINITY ? 0.f : v.z;
+  odd.w += fabsf(v.w) < INFINITY ? 0.f : v.w;
+}
+__device__ __forceinline__ void take_odd(float4& acc, float4 odd) {
+  acc.x = odd.x == 0.f ? acc.x : odd.x;
+  acc.y = odd.y == 0.f ? acc.y : odd.y;
+  acc.z = odd.z == 0.f ? acc.z : odd.z;
+  acc.w = odd.w == 0.f ? acc.w : odd.w;
+}
+
 // Tokens that a (sequence, KV head) unit of sequence b covers.
 __device__ __forceinline__ int unit_tokens(const PagedAttnParams& p, int b) {
   const int L = min(max(p.seq_lens[b], 0), p.max_len);
@@ -453,9 +478,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
           mma16816<T>(t0, pa, r[0], r[1]);
           mma16816<T>(t1, pa, r[2], r[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[2 * j][e] += t0[e];
-            o[2 * j + 1][e] += t1[e];
+          for (int e = 0; e < 4; e += 2) {
+            add2(o[2 * j][e], o[2 * j][e + 1], t0[e], t0[e + 1]);
+            add2(o[2 * j + 1][e], o[2 * j + 1][e + 1], t1[e], t1[e + 1]);
           }
         }
       }
@@ -507,6 +532,20 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
         acc.z += f * v.z;
         acc.w += f * v.w;
         l += f * red_l[w][row];
+      }
+      if (!finite4(acc) && l == l) {   // infinities or NaN in V
+        float4 odd = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int i = t0 << p.item_shift; i < end; ++i) {
+          int pos;
+          const int blk = locate(i, pos);
+          if (pos < 0) continue;
+          const int64_t at = ((int64_t)blk * p.v_s0 + (int64_t)(pos % p.block_size) * p.v_s1 + c) * 2;
+          const uint2 raw = *reinterpret_cast<const uint2*>(vbase + at);
+          const float2 a = unpack2(T{}, raw.x), b = unpack2(T{}, raw.y);
+          add_odd(odd, make_float4(a.x, a.y, b.x, b.y));
+        }
+        take_odd(acc, odd);
       }
       if (whole) {
         store_out<T>(p, b, head0 + row, c, acc, m, l);
@@ -627,6 +666,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttnParam
     acc.z += f * v.z;
     acc.w += f * v.w;
     l += f * ml.y;
+  }
+  if (!finite4(acc) && l == l) {
+    float4 odd = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i = i0; i <= i1; ++i)
+      add_odd(odd, *reinterpret_cast<const float4*>(part_slot(p, D, i, i == i0 && late) + row * D + col * 4));
+    take_odd(acc, odd);
   }
   store_out<T>(p, b, hk * p.group + hg * kRowsM + row, col * 4, acc, M, l);
 }
