@@ -54,6 +54,16 @@ class FullAttentionLayer:
         self.cos_sin_cache = cos_sin_cache
         self.q_norm, self.k_norm, self.eps, self.top_pages = q_norm, k_norm, eps, top_pages
         self.scale = HEAD_DIM ** -0.5
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.wqkv.device)
+
+    def read_status(self, reset: bool = True) -> int:
+        """The first device error that the layer's kernels recorded since the last reset, 0 if
+        none: 105 for a block id, slot or position outside its tensor, 106 for a wait that ran
+        out (the selection's lists are -1 then). Synchronises; also after a graph's replay."""
+        code = int(self.status)
+        if reset and code:
+            self.status.zero_()
+        return code
 
     def allocate_cache(self, num_blocks: int, block_size: int = 16) -> tuple:
         """(k_cache, v_cache), and the page bounds behind them with top_pages."""
@@ -71,7 +81,7 @@ class FullAttentionLayer:
         qkv = F.linear(hidden, self.wqkv).view(n, H + 2 * K, HEAD_DIM)
         q, k, v = qkv[:, :H], qkv[:, H:H + K], qkv[:, H + K:]
         q = qk_norm_rope_write(q, k, v, positions, self.cos_sin_cache, cache[0], cache[1], slot_mapping,
-                               q_weight=self.q_norm, k_weight=self.k_norm, eps=self.eps, k_out=k_out)
+                               q_weight=self.q_norm, k_weight=self.k_norm, eps=self.eps, k_out=k_out, status=self.status)
         return q, v
 
     def _o_proj(self, attn, reduce: bool):
@@ -88,10 +98,12 @@ class FullAttentionLayer:
         all-reduced over the group unless `reduce` is False."""
         q, _ = self._project(hidden, positions, cache, slot_mapping)
         if self.top_pages is None:
-            attn = pa.paged_attention_decode(q, cache[0], cache[1], block_table, seq_lens, max_seq_len, self.scale)
+            attn = pa.paged_attention_decode(q, cache[0], cache[1], block_table, seq_lens, max_seq_len, self.scale,
+                                             status=self.status)
         else:
-            pa.update_page_bounds(cache[0], cache[2], block_table, seq_lens, max_seq_len)
-            attn, _ = pa.sparse_paged_decode(q, *cache, block_table, seq_lens, max_seq_len, self.scale, self.top_pages)
+            pa.update_page_bounds(cache[0], cache[2], block_table, seq_lens, max_seq_len, status=self.status)
+            attn, _ = pa.sparse_paged_decode(q, *cache, block_table, seq_lens, max_seq_len, self.scale, self.top_pages,
+                                             status=self.status)
         return self._o_proj(attn, reduce)
 
     def prefill(self, hidden: torch.Tensor, positions: torch.Tensor, prompt_lens: list[int], cache: tuple,
@@ -110,8 +122,8 @@ class FullAttentionLayer:
         if self.top_pages is not None and T:
             longest = max(prompt_lens)
             lens = torch.tensor(prompt_lens, dtype=torch.int32, device=hidden.device)
-            pa.update_page_bounds(cache[0], cache[2], block_table, lens, longest, max_new=longest)
-        return self._o_proj(prefill_attention(q, k, v, prompt_lens, self.scale), reduce)
+            pa.update_page_bounds(cache[0], cache[2], block_table, lens, longest, max_new=longest, status=self.status)
+        return self._o_proj(prefill_attention(q, k, v, prompt_lens, self.scale, status=self.status), reduce)
 
 
 class FullContextLayer(FullAttentionLayer):
@@ -135,7 +147,7 @@ class FullContextLayer(FullAttentionLayer):
         describe its local sequences. Returns (out f32 undivided, m, l)."""
         q, _ = self._project(hidden, positions, cache, slot_mapping)
         return pa.paged_attention_decode(q, cache[0], cache[1], block_table, seq_lens, max_seq_len, self.scale,
-                                         return_partial=True)
+                                         return_partial=True, status=self.status)
 
     def forward(self, hidden, positions, cache, block_table, seq_lens, max_seq_len, slot_mapping, reduce: bool = True):
         """Decode step over this rank's pages, the exchange of the partials and o_proj; the
