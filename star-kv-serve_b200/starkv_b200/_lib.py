@@ -223,6 +223,12 @@ def addr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def refuse_status(what: str, status: torch.Tensor | None) -> None:
+    """The error for a status tensor that does not hold one aligned int32."""
+    if status is not None and (status.nbytes < 4 or status.data_ptr() & 3):
+        raise ValueError(f"{what}: status must hold an int32")
+
+
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 

@@ -54,6 +54,13 @@ def _tables(what: str, n: int, block_table: torch.Tensor, seq_lens: torch.Tensor
     return block_table, seq_lens
 
 
+def _refuse_memory(what: str, ws: torch.Tensor | None, status: torch.Tensor | None) -> None:
+    """The kernels write ws.nbytes in a row, and one aligned int32 of status."""
+    if ws is not None and not ws.is_contiguous():
+        raise ValueError(f"{what}: ws must be contiguous")
+    _lib.refuse_status(what, status)
+
+
 def _refuse_cache(what: str, name: str, cache: torch.Tensor, dtype: torch.dtype) -> None:
     """The error for a cache tensor that a call does not take, if it does not."""
     if cache.dim() != 4 or cache.shape[3] not in HEAD_DIMS or cache.stride(3) != 1:
@@ -101,7 +108,7 @@ def paged_attention_decode(
     views of one packed buffer (``partial``, allocated when not given; with head_dim 64,
     which ``combine`` does not take, three tensors).
 
-    ``ws``: scratch of this call alone (``workspace_bytes``); by default it is
+    ``ws``: contiguous scratch of this call alone (``workspace_bytes``); by default it is
     allocated on the current stream, so that calls that overlap, or captured graphs
     that are replayed at once, do not share it."""
     return _attend("paged_attention_decode", query, k_cache, v_cache, block_table, seq_lens, max_seq_len, scale, pages,
@@ -155,6 +162,7 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
     if out.data_ptr() == query.data_ptr() and n:
         raise ValueError(f"{what}: out may not be the query itself")
     bounds = None if select is None else select[0]
+    _refuse_memory(what, ws, status)
     idx = _lib.same_device(what, query, k_cache, v_cache, block_table, seq_lens, pages, out, ws, status, bounds)
     if n == 0:
         return (out, m, l) if return_partial else out
@@ -212,6 +220,7 @@ def update_page_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table:
         if new_lens.shape != (n,):
             raise ValueError(f"{what}: new_lens must be [{n}]")
         new_lens = new_lens.to(torch.int32).contiguous()
+    _refuse_memory(what, None, status)
     idx = _lib.same_device(what, k_cache, bounds, block_table, seq_lens, new_lens, status)
     a = _lib.pack_page_bounds(
         k_cache.data_ptr(), *k_cache.stride()[:3], bounds.data_ptr(), *bounds.stride()[:2], block_table.data_ptr(),
@@ -251,6 +260,7 @@ def select_pages(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.T
         out = seq_lens.new_empty((n, hkv, top))
     elif out.shape != (n, hkv, top) or out.dtype is not torch.int32 or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must be int32 [{n}, {hkv}, {top}], last dimension contiguous")
+    _refuse_memory(what, ws, status)
     idx = _lib.same_device(what, query, bounds, block_table, seq_lens, out, ws, status)
     if n == 0:
         return out

@@ -85,6 +85,7 @@ def _run(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping
     if k_out is not None:
         kos = _rows(what, "k_out", k_out, k_sizes, dtype)
     positions = positions.contiguous()
+    _lib.refuse_status(what, status)
     idx = _lib.same_device(what, q, k, v, positions, cos_sin_cache, k_cache, v_cache, slot_mapping, q_weight, k_weight,
                            q_out, k_out, status)
     if n == 0:
