@@ -40,6 +40,7 @@ def empty_bounds(k_cache: torch.Tensor) -> torch.Tensor:
 
 
 _CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}   # the cache's element types
+_LONGEST = 1 << 30   # tokens of a sequence that a call takes; any larger bound means this one
 
 
 def _tables(what: str, n: int, block_table: torch.Tensor, seq_lens: torch.Tensor):
@@ -162,20 +163,21 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
     if out.data_ptr() == query.data_ptr() and n:
         raise ValueError(f"{what}: out may not be the query itself")
     bounds = None if select is None else select[0]
+    max_seq_len = min(int(max_seq_len), _LONGEST)
     _refuse_memory(what, ws, status)
     idx = _lib.same_device(what, query, k_cache, v_cache, block_table, seq_lens, pages, out, ws, status, bounds)
     if n == 0:
         return (out, m, l) if return_partial else out
     if ws is None:
-        need = workspace_bytes(hq, hkv, d, top * bs if top else int(max_seq_len))
+        need = workspace_bytes(hq, hkv, d, top * bs if top else max_seq_len)
         if select is not None:
-            need += select_workspace_bytes(n, hkv, int(max_seq_len), bs, top)
+            need += select_workspace_bytes(n, hkv, min(max_seq_len, block_table.shape[1] * bs), bs, top)
         ws = seq_lens.new_empty((need + 3) // 4) if need else None
     P = _lib.addr
     a = _lib.pack_paged_attn(
         query.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
         block_table.data_ptr(), *block_table.stride(), seq_lens.data_ptr(), P(pages), *pg, out.data_ptr(),
-        *out.stride()[:2], P(m), P(l), P(status), _CODES[dtype], n, hq, hkv, d, nb, bs, block_table.shape[1], int(max_seq_len), top, float(scale))
+        *out.stride()[:2], P(m), P(l), P(status), _CODES[dtype], n, hq, hkv, d, nb, bs, block_table.shape[1], max_seq_len, top, float(scale))
     size = 0 if ws is None else ws.nbytes
     if select is None:
         _lib.launch(what, idx, _lib.lib().starkv_paged_attention, a, P(ws), size)
@@ -189,14 +191,14 @@ def _attend(what, query, k_cache, v_cache, block_table, seq_lens, max_seq_len, s
 def workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int, max_tokens: int) -> int:
     """Scratch of one ``paged_attention_decode`` over at most ``max_tokens`` tokens per sequence."""
     return int(_lib.lib().starkv_paged_attention_workspace_bytes(num_heads, num_kv_heads, head_dim,
-                                                                  min(int(max_tokens), 1 << 30)))
+                                                                  min(int(max_tokens), _LONGEST)))
 
 
 @lru_cache(maxsize=256)
 def select_workspace_bytes(n: int, num_kv_heads: int, max_seq_len: int, block_size: int, top: int) -> int:
     """Scratch of one ``select_pages``; ``sparse_paged_decode`` takes this and ``workspace_bytes``
     of top * block_size tokens."""
-    return int(_lib.lib().starkv_select_pages_workspace_bytes(n, num_kv_heads, min(int(max_seq_len), 1 << 30),
+    return int(_lib.lib().starkv_select_pages_workspace_bytes(n, num_kv_heads, min(int(max_seq_len), _LONGEST),
                                                               block_size, top))
 
 
@@ -225,7 +227,7 @@ def update_page_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table:
     a = _lib.pack_page_bounds(
         k_cache.data_ptr(), *k_cache.stride()[:3], bounds.data_ptr(), *bounds.stride()[:2], block_table.data_ptr(),
         *block_table.stride(), seq_lens.data_ptr(), _lib.addr(new_lens), _lib.addr(status), _CODES[k_cache.dtype],
-        n, hkv, d, nb, bs, block_table.shape[1], int(max_seq_len), int(max_new))
+        n, hkv, d, nb, bs, block_table.shape[1], min(int(max_seq_len), _LONGEST), min(int(max_new), _LONGEST))
     _lib.launch(what, idx, _lib.lib().starkv_page_bounds, a)
 
 
@@ -260,17 +262,18 @@ def select_pages(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.T
         out = seq_lens.new_empty((n, hkv, top))
     elif out.shape != (n, hkv, top) or out.dtype is not torch.int32 or out.stride(-1) != 1:
         raise ValueError(f"{what}: out must be int32 [{n}, {hkv}, {top}], last dimension contiguous")
+    max_seq_len = min(int(max_seq_len), _LONGEST)
     _refuse_memory(what, ws, status)
     idx = _lib.same_device(what, query, bounds, block_table, seq_lens, out, ws, status)
     if n == 0:
         return out
     if ws is None:
-        need = select_workspace_bytes(n, hkv, max_seq_len, block_size, top)
+        need = select_workspace_bytes(n, hkv, min(max_seq_len, block_table.shape[1] * block_size), block_size, top)
         ws = seq_lens.new_empty((need + 3) // 4) if need else None
     a = _lib.pack_select_pages(
         query.data_ptr(), *query.stride()[:2], bounds.data_ptr(), *bounds.stride()[:2], block_table.data_ptr(),
         *block_table.stride(), seq_lens.data_ptr(), out.data_ptr(), *out.stride()[:2], _lib.addr(status),
-        _CODES[query.dtype], n, hq, hkv, d, nb, int(block_size), block_table.shape[1], int(max_seq_len), int(top),
+        _CODES[query.dtype], n, hq, hkv, d, nb, int(block_size), block_table.shape[1], max_seq_len, int(top),
         int(sinks), int(recent))
     _lib.launch(what, idx, _lib.lib().starkv_select_pages, a, _lib.addr(ws), 0 if ws is None else ws.nbytes)
     return out
