@@ -9,7 +9,7 @@ for chance.
 import pytest
 import torch
 
-from test_gpu_paged_attention import make, tokens_of
+from test_gpu_paged_attention import check, make, reference, tokens_of
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,71 @@ def test_outputs_are_the_nearest_as_often_as_with_f32(lens, H, Hkv, dtype):
             off += int((got[b, r] != nearest).sum())
             off32 += int((plain(q[b, r], K[:, h], V[:, h], scale, torch.float32).to(dtype) != nearest).sum())
     assert off <= off32 + 4 * off32 ** 0.5, (off, off32, got.numel())
+
+
+def exact_partial(q, K, V, scale):
+    """(out undivided, m, l) of one KV head in float64."""
+    x = scale * (q.double() @ K.double().T)
+    m = x.amax(-1)
+    w = torch.exp(x - m[:, None])
+    return w @ V.double(), m, w.sum(-1)
+
+
+@pytest.mark.parametrize("H,Hkv,D,dtype,L", [
+    (8, 2, 128, torch.bfloat16, 131071), (12, 1, 128, torch.bfloat16, 40001), (17, 1, 128, torch.bfloat16, 9000),
+    (40, 1, 64, torch.bfloat16, 20011), (4, 2, 64, torch.bfloat16, 50000), (12, 1, 128, torch.float16, 40001),
+    (3, 3, 64, torch.float16, 30001)])
+@pytest.mark.parametrize("listed", [False, True])
+def test_partial_form_in_norm(H, Hkv, D, dtype, L, listed):
+    """Long, rather flat softmax, whole and over every other page, split and joined. The error
+    of a head's out and l, in norm: some hundred f32 additions one after another, whose
+    roundings add up as a root (10 2^-24), the hardware exponential (2^-22 at most), the
+    logits' and the maximum's error (128 products in f32, a few 2^-24 of logits of a few):
+    below 2^-20 together. bf16 weights in two parts, or sums that cut off, are above it."""
+    from starkv_b200.kernels.paged_attention import paged_attention_decode
+    q, k, v, bt, sl = make([L], H, Hkv, D=D, dtype=dtype, seed=H + L)
+    scale, G, bs = D ** -0.5, H // Hkv, 16
+    P = -(-L // bs)
+    pages = torch.arange(0, P, 2, dtype=torch.int32, device=q.device).expand(1, Hkv, -1) if listed else None
+    out, m, l = paged_attention_decode(q, k, v, bt, sl, L, scale, pages=pages, return_partial=True)
+    t = torch.arange(L, device=q.device)
+    if listed:
+        t = t[t // bs % 2 == 0]
+    K, V = tokens_of(k, bt[0], t), tokens_of(v, bt[0], t)
+    for h in range(Hkv):
+        r = slice(h * G, (h + 1) * G)
+        ro, rm, rl = exact_partial(q[0, r], K[:, h], V[:, h], scale)
+        assert ((out[0, r].double() - ro).norm(dim=-1) <= 2.0 ** -20 * ro.norm(dim=-1)).all(), \
+            float(((out[0, r].double() - ro).norm(dim=-1) / ro.norm(dim=-1)).max())
+        assert ((l[0, r].double() - rl).abs() <= 2.0 ** -20 * rl).all()
+        assert ((m[0, r].double() - rm).abs() <= 2.0 ** -20 * rm.abs().clamp(min=1)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,Hkv,D", [(12, 1, 128), (17, 1, 128), (40, 1, 64), (32, 2, 128), (8, 2, 64), (3, 3, 64)])
+@pytest.mark.parametrize("listed", [False, True])
+def test_partial_form_at_edge_lengths(H, Hkv, D, dtype, listed):
+    from starkv_b200.kernels.paged_attention import paged_attention_decode
+    lens = [1, 0, 15, 16, 17, 64, 65, 256, 257, 1003]
+    q, k, v, bt, sl = make(lens, H, Hkv, D=D, dtype=dtype, seed=D + H)
+    scale, pages = D ** -0.5, None
+    if listed:   # any order, a hole among them, 14 pages at most
+        g = torch.Generator().manual_seed(H)
+        pages = torch.full((len(lens), Hkv, 14), -1, dtype=torch.int32)
+        for b, L in enumerate(lens):
+            P = -(-L // 16)
+            for h in range(Hkv):
+                c = min(14, P)
+                pages[b, h, :c] = torch.randperm(P, generator=g)[:c].int()
+                if c > 3:
+                    pages[b, h, 1] = -1
+        pages = pages.to(q.device)
+    out, m, l = paged_attention_decode(q, k, v, bt, sl, 1003, scale, pages=pages, return_partial=True)
+    ref, rm, rl, tol = reference(q, k, v, bt, sl, scale, pages=pages)
+    empty = rl == 0
+    assert (m[empty] == float("-inf")).all() and (l[empty] == 0).all() and (out[empty] == 0).all()
+    assert empty.any() and not empty.all()
+    live = ~empty
+    assert ((m - rm)[live].abs() <= tol[..., 0][live]).all()
+    assert ((l - rl)[live].abs() <= 2 * tol[..., 0][live] * rl[live]).all()
+    check((out / l[..., None])[live], ref[live], 2 * tol[live])
