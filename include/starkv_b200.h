@@ -328,12 +328,16 @@ STARKV_API int starkv_page_bounds(const StarKVPageBoundsArgs* args, void* stream
 
 /*
  * The `top` pages per (sequence, KV head) with the highest
- *   sum over the head's query heads g and channels d of max(q[g,d] lo[d], q[g,d] hi[d]),
+ *   sum over the channels d of up[d] hi[d] + down[d] lo[d],
+ *   up[d] = sum over the head's query heads g of max(q[g,d], 0), down[d] that of min(q[g,d], 0),
+ * which for finite lo <= hi is the sum over g and d of max(q[g,d] lo[d], q[g,d] hi[d]),
  * ascending, -1 behind them where the sequence has fewer pages: pages int32
  * [n, num_kv_heads, top] (strides {sequence, head}). The first `sinks` and the last
  * `recent` pages of a sequence are always among them (sinks >= 0, recent >= 0,
  * sinks + recent <= top); their bounds are not read. Scores in 64 bits, ties to the
- * lowest page, a NaN score above all others. The workspace (16-byte aligned, may be null
+ * lowest page, a NaN score above all others. NaN is also what an infinite bound gives on a
+ * side whose up or down is 0: a page whose keys overflowed that way is always taken before
+ * the others, never hidden. The workspace (16-byte aligned, may be null
  * where its size is 0; max_tokens: min(max_seq_len, max_blocks * block_size)) is scratch
  * of this call alone.
  */

@@ -3,7 +3,8 @@
 // (G = query heads per KV head), over all tokens or over a list of pages per (sequence,
 // KV head).
 //
-// What bounds it: every K and V row is read once and used for G heads, 4 G FLOP per
+// What bounds it: a K or V row is read once for up to 16 query heads (the M of an MMA; more
+// heads of a KV head are units of their own, which read it again), 4 FLOP per head and
 // element of 2 bytes, so the cache read is the cost. The tokens of all (sequence, KV
 // head) units are laid end to end in items of 64 tokens and every CTA of one wave takes an
 // equal run of them, whatever the mix of lengths. A unit that lies inside one CTA's run

@@ -8,7 +8,9 @@
 //   score(page) = sum_{g in group} sum_d max(q[g, d] lo[d], q[g, d] hi[d])
 //               = sum_d up[d] hi[d] + down[d] lo[d],
 //   up = sum_g max(q[g], 0),  down = sum_g min(q[g], 0),
-// an upper bound of sum_g q[g] . k over the page's keys. One page costs 4 D bytes and 2 D
+// an upper bound of sum_g q[g] . k over the page's keys. The second form is the definition
+// where a bound is infinite: on a side of weight 0 it gives NaN, which ranks first, so that a
+// page whose keys overflowed is read and not hidden. One page costs 4 D bytes and 2 D
 // multiply-adds whatever G is, so the read of the bounds is the cost.
 //
 // The selection is that of scores summed in 64 bits (products of two 16-bit values are

@@ -248,12 +248,16 @@ def select_pages(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.T
                  max_seq_len: int, block_size: int, top: int, *, sinks: int = 1, recent: int = 1,
                  out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
                  status: torch.Tensor | None = None) -> torch.Tensor:
-    """The ``top`` pages per sequence and KV head with the largest
-    ``sum_{g, d} max(q[g, d] lo[d], q[g, d] hi[d])`` over the head's query heads g:
+    """The ``top`` pages per sequence and KV head with the largest score
+    ``sum_d up[d] hi[d] + down[d] lo[d]``, ``up = sum_g max(q[g], 0)`` and ``down = sum_g min(q[g], 0)``
+    over the head's query heads g (for finite lo <= hi this is
+    ``sum_{g, d} max(q[g, d] lo[d], q[g, d] hi[d])``):
     int32 [n, H_kv, top], ascending, -1 behind them where a sequence has fewer pages.
     The first ``sinks`` and the last ``recent`` pages are always among them (the last
     page is usually not full, and its bounds need not be up to date while recent >= 1).
-    Scores in 64 bits; ties go to the lowest page; a NaN score ranks above all others."""
+    Scores in 64 bits; ties go to the lowest page; a NaN score ranks above all others, also
+    that of an infinite bound on a side whose ``up`` or ``down`` is 0: a page whose keys
+    overflowed that way is taken first."""
     what = "select_pages"
     nb, hkv, d = _check_bounds(what, query, bounds, top, sinks, recent)
     n, hq, _ = _query_sizes(what, query, hkv, d)
