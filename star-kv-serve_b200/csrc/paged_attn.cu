@@ -22,12 +22,13 @@
 // sums.
 //
 // The weights and the output keep the precision of f32 all the way. P is split into parts
-// of the cache's type, bf16 into three (24 bits), f16 into two (22 bits); with G <= 8 the
-// first two share one MMA (rows 0-7 and 8-15). The tensor core's own accumulation cuts
-// off instead of rounding, so an MMA of P V adds to zero and its result to the sum by a
-// rounded f32 addition. (24 x 8192 tokens, 32 / 32 heads, bf16, two parts and the tensor
+// of the cache's type, bf16 into three (24 bits), f16 into two (22 bits). With G <= 8 the
+// first two share one MMA (rows 0-7 and 8-15), with G <= 4 all three (rows 0-3, 8-11 and
+// 4-7, whose scores come from the queries of rows 0-3 once more). The tensor core's own
+// accumulation cuts off instead of rounding, so an MMA of P V adds to zero and its result
+// to the sum by a rounded f32 addition. (24 x 8192 tokens, 32 / 32 heads, bf16, two parts and the tensor
 // core's sums: 2.4 of 1000 outputs were not the nearest to the exact value, against 1.0 of
-// 1000 with f32 operations and 0.5 this way, at the same time.)
+// 1000 with f32 operations and 0.5 this way.)
 #include <algorithm>
 #include <type_traits>
 
@@ -45,8 +46,8 @@ constexpr int kSub = 16;                 // tokens of a warp's share of a tile
 constexpr int kTileTok = kWarps * kSub;  // tokens of a tile
 constexpr int kTileShift = 6, kWholeShift = 8;
 // Units of at most this many tokens are not split and not joined (8 KV heads, 256 tokens:
-// one sequence 7.9 against 6.9 us but a launch less for the host, 64 sequences 15.7 against
-// 20.0; at 512 tokens one sequence takes 11.6 us whole and 7.1 split).
+// one sequence 7.4 us whole and 7.0 split but a launch less for the host, 8 sequences 7.6 and
+// 9.3, 64 sequences 15.6 and 20.1; 512 tokens: 10.7 and 7.1, 11.1 and 11.8, 29.5 and 31.6).
 constexpr int kWholeTokens = 1 << kWholeShift;
 constexpr int kStages = 3;
 constexpr int kMaxShares = 384;          // CTAs of one call at most
@@ -202,11 +203,13 @@ __device__ __forceinline__ void store_out(const PagedAttnParams& p, int b, int h
   store4(reinterpret_cast<T*>(p.out) + at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
-// kTwo: more than 8 query heads in the unit's MMA rows. kF32: the partial form, whose
+// kHeads: 4, 8 or 16, the most query heads of a unit; 4 for bf16 alone (a third MMA for the
+// third part: 24 x 8192 tokens of 32 / 32 heads back to back under the power cap 542 us, in
+// one MMA 488; 2 parts 483). kF32: the partial form, whose
 // output is f32 and shows what 16 bits hide: the MMAs of Q K^T add to zero as well
 // (131071 tokens: 4.8e-7 off, relative in norm, against 6.1e-7). Not where the output is
 // rounded to 16 bits: one sequence of 201 tokens 8.4 us, with it 9.1.
-template <typename T, int D, bool kTwo, bool kSparse, bool kF32>
+template <typename T, int D, int kHeads, bool kSparse, bool kF32>
 __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttnParams p) {
   using R = Ring<D>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -219,7 +222,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   const uint32_t ring = smem_u32(smem) + warp * R::warp_bytes;
   const float c_log2 = p.scale * 1.4426950408889634f;
   constexpr float kBias = weight_bias<T>();
+  constexpr bool kTwo = kHeads > 8, kFour = kHeads <= 4;
   constexpr bool kThird = std::is_same<T, __nv_bfloat16>::value;
+  static_assert(!kFour || kThird, "rows 4-7 hold the third part");
 
   // the joining kernel's blocks may take the place of CTAs that are done; they wait for all
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -265,10 +270,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
 #pragma unroll
       for (int kk = 0; kk < kKSteps; ++kk) {
         const int d = kk * 16 + 2 * qc;
-        const T* r0 = q + (int64_t)qr * p.q_s1 + d;
+        const int row0 = kFour ? qr & 3 : qr;
+        const T* r0 = q + (int64_t)row0 * p.q_s1 + d;
         const T* r1 = q + (int64_t)(qr + 8) * p.q_s1 + d;
-        qa[kk][0] = qr < rows ? *reinterpret_cast<const uint32_t*>(r0) : 0u;
-        qa[kk][2] = qr < rows ? *reinterpret_cast<const uint32_t*>(r0 + 8) : 0u;
+        qa[kk][0] = row0 < rows ? *reinterpret_cast<const uint32_t*>(r0) : 0u;
+        qa[kk][2] = row0 < rows ? *reinterpret_cast<const uint32_t*>(r0 + 8) : 0u;
         qa[kk][1] = kTwo && qr + 8 < rows ? *reinterpret_cast<const uint32_t*>(r1) : 0u;
         qa[kk][3] = kTwo && qr + 8 < rows ? *reinterpret_cast<const uint32_t*>(r1 + 8) : 0u;
       }
@@ -458,6 +464,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
           pt[1] = t1a;
           pt[3] = t3a;
         }
+        if (kFour && qr >= 4) {
+          pa[0] = pt[0];
+          pa[1] = 0u;
+          pa[2] = pt[2];
+          pa[3] = 0u;
+        }
       }
       // ---- O += P V ----
       {
@@ -468,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
           uint32_t r[4];
           ldsm4_t(a + (((2 * j + (mi >> 1)) ^ rr) << 4), r);
           float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
-          if (kThird) {   // the smallest part first
+          if (kThird && !kFour) {   // the smallest part first
             mma16816<T>(t0, pt, r[0], r[1]);
             mma16816<T>(t1, pt, r[2], r[3]);
           }
@@ -506,6 +518,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
       if (!kTwo) {
         o[j][0] += o[j][2];
         o[j][1] += o[j][3];
+        if (kFour) {
+          o[j][0] += __shfl_xor_sync(~0u, o[j][0], 16);
+          o[j][1] += __shfl_xor_sync(~0u, o[j][1], 16);
+        }
       }
       if (qr < rows)
         *reinterpret_cast<float2*>(red + (warp * kRowsM + qr) * D + j * 8 + 2 * qc) = make_float2(o[j][0], o[j][1]);
@@ -678,20 +694,18 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttnParam
   store_out<T>(p, b, hk * p.group + hg * kRowsM + row, col * 4, acc, M, l);
 }
 
-template <typename T, int D, bool kSparse>
-const void* attn_fn(bool two, bool f32) {
-  if (f32)
-    return two ? (const void*)paged_attn_kernel<T, D, true, kSparse, true>
-               : (const void*)paged_attn_kernel<T, D, false, kSparse, true>;
-  return two ? (const void*)paged_attn_kernel<T, D, true, kSparse, false>
-             : (const void*)paged_attn_kernel<T, D, false, kSparse, false>;
+template <typename T, int D, bool kSparse, bool kF32>
+const void* attn_fn(int group) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    if (group <= 4) return (const void*)paged_attn_kernel<T, D, 4, kSparse, kF32>;
+  return group <= 8 ? (const void*)paged_attn_kernel<T, D, 8, kSparse, kF32>
+                    : (const void*)paged_attn_kernel<T, D, 16, kSparse, kF32>;
 }
 
 template <typename T, int D>
 int launch_typed(const PagedAttnParams& p, int num_sms, cudaStream_t stream) {
-  const bool two = p.group > 8;
-  const bool f32 = p.m_out != nullptr;
-  const void* fn = p.pages ? attn_fn<T, D, true>(two, f32) : attn_fn<T, D, false>(two, f32);
+  const void* fn = p.pages ? p.m_out ? attn_fn<T, D, true, true>(p.group) : attn_fn<T, D, true, false>(p.group)
+                   : p.m_out ? attn_fn<T, D, false, true>(p.group) : attn_fn<T, D, false, false>(p.group);
   const int smem = Ring<D>::bytes;
   if (const int st = allow_smem(fn, smem)) return st;
   PagedAttnParams q = p;
