@@ -21,14 +21,19 @@
 // end are filled with zeros by the copy itself, so whatever they hold cannot reach the
 // sums.
 //
-// The weights and the output keep the precision of f32 all the way. P is split into parts
-// of the cache's type, bf16 into three (24 bits), f16 into two (22 bits). With G <= 8 the
-// first two share one MMA (rows 0-7 and 8-15), with G <= 4 all three (rows 0-3, 8-11 and
-// 4-7, whose scores come from the queries of rows 0-3 once more). The tensor core's own
-// accumulation cuts off instead of rounding, so an MMA of P V adds to zero and its result
-// to the sum by a rounded f32 addition. (24 x 8192 tokens, 32 / 32 heads, bf16, two parts and the tensor
-// core's sums: 2.4 of 1000 outputs were not the nearest to the exact value, against 1.0 of
-// 1000 with f32 operations and 0.5 this way.)
+// Precision of the weights and of the sums. P is split into parts of the cache's type, so
+// that its rounding (2^-9 for bf16) does not show. With G <= 8 two parts share one MMA (rows
+// 0-7 and 8-15), with G <= 4 three do (rows 0-3, 8-11 and 4-7, whose scores come from the
+// queries of rows 0-3 once more). The tensor core's own accumulation cuts off instead of
+// rounding. Shares of outputs that are not the nearest to the exact value, of 1000:
+//   f16 in two parts (22 bits), sums of the tensor core                 4.2, f32 operations 7.0
+//   bf16, G <= 4: three parts (24 bits), every MMA of P V added to zero
+//     and its result to the sum by a rounded f32 addition               0.5, f32 operations 1.0
+//     (in two parts and by the tensor core's sums 2.4, at the same time)
+//   bf16, G > 4: two parts (16 bits), sums of the tensor core           1.6, f32 operations 0.9
+//     (as above, with a third MMA: 0.4, but 192 against 168 us for 32 x 8160 tokens of 64 / 8
+//     heads, 116 against 95 with heads of 64: not worth a last place of a bf16 in a thousand)
+// The partial form, whose output is f32, is always of the second kind.
 #include <algorithm>
 #include <type_traits>
 
@@ -203,12 +208,11 @@ __device__ __forceinline__ void store_out(const PagedAttnParams& p, int b, int h
   store4(reinterpret_cast<T*>(p.out) + at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
-// kHeads: 4, 8 or 16, the most query heads of a unit; 4 for bf16 alone (a third MMA for the
-// third part: 24 x 8192 tokens of 32 / 32 heads back to back under the power cap 542 us, in
-// one MMA 488; 2 parts 483). kF32: the partial form, whose
-// output is f32 and shows what 16 bits hide: the MMAs of Q K^T add to zero as well
-// (131071 tokens: 4.8e-7 off, relative in norm, against 6.1e-7). Not where the output is
-// rounded to 16 bits: one sequence of 201 tokens 8.4 us, with it 9.1.
+// kHeads: 4, 8 or 16, the most query heads of a unit; 4 for bf16 alone (24 x 8192 tokens of
+// 32 / 32 heads back to back under the power cap: three parts in one MMA 488 us, the third
+// in one of its own 542, two parts 483). kF32: the partial form; the MMAs of Q K^T add to
+// zero as well (131071 tokens: 4.8e-7 off, relative in norm, against 6.1e-7), which does not
+// show in 16 bits (the 24 x 8192 tokens 483 us, with it 495).
 template <typename T, int D, int kHeads, bool kSparse, bool kF32>
 __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttnParams p) {
   using R = Ring<D>;
@@ -223,8 +227,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
   const float c_log2 = p.scale * 1.4426950408889634f;
   constexpr float kBias = weight_bias<T>();
   constexpr bool kTwo = kHeads > 8, kFour = kHeads <= 4;
-  constexpr bool kThird = std::is_same<T, __nv_bfloat16>::value;
-  static_assert(!kFour || kThird, "rows 4-7 hold the third part");
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool kRounded = kFour || kF32, kThird = kRounded && kBf16;
+  static_assert(!kFour || kBf16, "rows 4-7 hold the third part");
 
   // the joining kernel's blocks may take the place of CTAs that are done; they wait for all
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -480,20 +485,24 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const PagedAttn
           uint32_t r[4];
           ldsm4_t(a + (((2 * j + (mi >> 1)) ^ rr) << 4), r);
           float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+          float(&x)[4] = kRounded ? t0 : o[2 * j];
+          float(&y)[4] = kRounded ? t1 : o[2 * j + 1];
           if (kThird && !kFour) {   // the smallest part first
-            mma16816<T>(t0, pt, r[0], r[1]);
-            mma16816<T>(t1, pt, r[2], r[3]);
+            mma16816<T>(x, pt, r[0], r[1]);
+            mma16816<T>(y, pt, r[2], r[3]);
           }
           if (kTwo) {
-            mma16816<T>(t0, pl, r[0], r[1]);
-            mma16816<T>(t1, pl, r[2], r[3]);
+            mma16816<T>(x, pl, r[0], r[1]);
+            mma16816<T>(y, pl, r[2], r[3]);
           }
-          mma16816<T>(t0, pa, r[0], r[1]);
-          mma16816<T>(t1, pa, r[2], r[3]);
+          mma16816<T>(x, pa, r[0], r[1]);
+          mma16816<T>(y, pa, r[2], r[3]);
+          if (kRounded) {
 #pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            add2(o[2 * j][e], o[2 * j][e + 1], t0[e], t0[e + 1]);
-            add2(o[2 * j + 1][e], o[2 * j + 1][e + 1], t1[e], t1[e + 1]);
+            for (int e = 0; e < 4; e += 2) {
+              add2(o[2 * j][e], o[2 * j][e + 1], t0[e], t0[e + 1]);
+              add2(o[2 * j + 1][e], o[2 * j + 1][e + 1], t1[e], t1[e + 1]);
+            }
           }
         }
       }

@@ -5,6 +5,14 @@ error crosses a rounding border, so the share of such outputs measures that erro
 not be larger than that of the same formula in elementary f32 operations. Both shares are
 counts of rare independent events; 4 square roots of the larger expected count are left
 for chance.
+
+bf16 with more than 4 query heads per KV head: the weights keep two parts of 8 bits, which
+leave at most 2^-18 of a weight, evenly spread: 2^-18 / sqrt(3) rms, and as much of the
+output's own size s in norm, since V has both signs. An output x is not the nearest with
+probability |error| / step(x). Outputs are about normal; step(x) = 2^-7 2^k in the binade
+[2^k, 2^k+1), each binade below s holds 0.8 2^k / s of the outputs, and the first 12 below s
+have steps above the error, so the mean of s / step is 2^7 (12 0.8 + 1), that of |error| is
+0.8 2^-18 / sqrt(3) s: 0.8 2^-11 10.6 / sqrt(3) = 2.4e-3 of the outputs on top of f32's.
 """
 import pytest
 import torch
@@ -22,7 +30,8 @@ def plain(q, K, V, scale, dtype):
 
 
 @pytest.mark.parametrize("lens,H,Hkv,dtype", [([8192] * 12, 32, 32, torch.bfloat16), ([8000] * 12, 64, 8, torch.bfloat16),
-                                              ([7001] * 6, 96, 8, torch.bfloat16), ([8191] * 12, 32, 8, torch.float16)])
+                                              ([7001] * 6, 96, 8, torch.bfloat16), ([8191] * 12, 32, 8, torch.float16),
+                                              ([8191] * 12, 32, 8, torch.bfloat16), ([6000] * 12, 64, 8, torch.float16)])
 def test_outputs_are_the_nearest_as_often_as_with_f32(lens, H, Hkv, dtype):
     from starkv_b200.kernels.paged_attention import paged_attention_decode
     q, k, v, bt, sl = make(lens, H, Hkv, dtype=dtype, seed=90 + Hkv, qmag=1.7)
@@ -37,6 +46,8 @@ def test_outputs_are_the_nearest_as_often_as_with_f32(lens, H, Hkv, dtype):
             nearest = plain(q[b, r], K[:, h], V[:, h], scale, torch.float64).to(dtype)
             off += int((got[b, r] != nearest).sum())
             off32 += int((plain(q[b, r], K[:, h], V[:, h], scale, torch.float32).to(dtype) != nearest).sum())
+    if dtype == torch.bfloat16 and G > 4:
+        off32 += 0.8 * 2 ** -11 * 10.6 / 3 ** 0.5 * got.numel()
     assert off <= off32 + 4 * off32 ** 0.5, (off, off32, got.numel())
 
 
