@@ -962,8 +962,8 @@ int launch_select_typed(SelectPagesParams p, int num_sms, cudaStream_t stream) {
   cfg.attrs = attr;
   // One kernel where a CTA per unit, one to an SM, is enough for the reads. Its time grows
   // with the pages of a unit, that of two kernels with all pages: 8 units of 128 / 375 / 512
-  // / 1024 pages 7.2 / 8.9 / 12.0 / 15.9 us against 9.5 / 9.1 / 10.3 / 10.0 in two; 128 units
-  // of 256 / 512 pages 9.3 / 11.4 against 12.2 / 14.4. The launch less is 4 us of the host's.
+  // / 1024 pages 7.2 / 8.9 / 11.5 / 15.8 us against 9.4 / 9.1 / 10.3 / 10.0 in two; 128 units
+  // of 256 / 512 pages 9.3 / 11.5 against 12.2 / 15.0. The launch less is 4 us of the host's.
   if (units <= num_sms && p.key_stride <= kFusedPages) {
     const void* fn = (const void*)pick_kernel<T, D, kFusedThreads, true>;
     if (const int st = allow_smem(fn, ring_bytes(kFusedThreads))) return st;
